@@ -9,22 +9,19 @@
 #include <cstring>
 #include <mutex>
 
+#include "gemm_host.cuh"
 #include "gemm_simt.cuh"
 #include "gemm_sm100.cuh"
 #include "gemm_sm100_2sm.cuh"
 #include "gemm_sm100_sk.cuh"
 
-namespace {
-
-using col::sm100::GemmParams;
-using col::sm100::TileCfg;
-
 // Device-side status word of the bounded waits (one per device context).
-__device__ unsigned g_gemm_status;
+static __device__ unsigned g_gemm_status;
 
-constexpr int kMaxDevices = 64;
+namespace col {
 
-unsigned* status_ptr(int dev) {
+unsigned* gemm_status_ptr(int dev) {
+  constexpr int kMaxDevices = 64;
   static unsigned* ptrs[kMaxDevices] = {};
   static std::once_flag flags[kMaxDevices];
   std::call_once(flags[dev], [dev]() {
@@ -48,6 +45,13 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   });
   return fn;
 }
+
+}  // namespace col
+
+namespace {
+
+using col::sm100::GemmParams;
+using col::sm100::TileCfg;
 
 // Recently encoded tensor maps of the calling thread.  A map is a pure
 // function of (base, rows, cols, box_rows) -- the element type, swizzle, L2
@@ -76,7 +80,7 @@ int encode_bf16_rows(CUtensorMap* map, const void* base, std::uint64_t rows, std
     std::memcpy(map, &e.map, sizeof(CUtensorMap));
     return 0;
   }
-  auto enc = tensor_map_encoder();
+  auto enc = col::tensor_map_encoder();
   if (!enc) return col::kErrNoTensorMapEncoder;
   const cuuint64_t dims[2] = {cols, rows};
   const cuuint64_t strides[1] = {cols * 2};
@@ -311,7 +315,7 @@ int launch_tensor_gemm(const TcOperands& ops, BMode mode, const float* bias, voi
   int dev = 0;
   const col::DeviceInfo& info = col::device_info(&dev);
   if (info.cc_major != 10) return col::kErrDeviceNotSupported;
-  unsigned* status = status_ptr(dev);
+  unsigned* status = col::gemm_status_ptr(dev);
   if (!status) return static_cast<int>(cudaErrorInvalidDevice);
 
   const int mblocks = static_cast<int>((m + 127) / 128);

@@ -89,6 +89,20 @@ _SIGNATURES["cuda_operator_lab_peer_status"] = [_P, _I32]
 _SIGNATURES["cuda_operator_lab_device_info"] = [_P, _P, _P]
 _SIGNATURES["cuda_operator_lab_build_tag"] = []
 _SIGNATURES["cuda_operator_lab_gemm_status"] = [_P, _I32]
+# e4m3 block-128 operands and products grouped by expert (fp8.py, grouped.py)
+for _v in ("f32", "bf16"):
+    _SIGNATURES[f"cuda_operator_quantize_fp8_block128_{_v}"] = [_P, _P, _P, _U64, _U64, _P]
+    _SIGNATURES[f"cuda_operator_quantize_fp8_block128_weight_{_v}"] = [
+        _P, _P, _P, _U64, _U64, _U64, _P]
+for _v in ("gemm", "gemm_swiglu"):
+    _SIGNATURES[f"cuda_operator_{_v}_fp8_block128"] = [_P, _P, _P, _P, _P, _U64, _U64, _U64, _P]
+for _v in ("gemm_grouped", "gemm_grouped_swiglu"):
+    _SIGNATURES[f"cuda_operator_{_v}_bf16"] = [_P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]
+    _SIGNATURES[f"cuda_operator_{_v}_fp8_block128"] = [
+        _P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]
+for _v in ("input", "weight"):
+    _SIGNATURES[f"cuda_operator_gemm_grouped_bf16_grad_{_v}"] = [
+        _P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]
 _SIGNATURES["cuda_operator_lab_reduction_noalloc"] = [_P, _P, _U64, _P]
 
 _RESTYPES = {

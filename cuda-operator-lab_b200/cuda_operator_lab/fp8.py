@@ -1,0 +1,230 @@
+"""8-bit (e4m3) operands with a scale for each block of 128, and their products.
+
+A matrix is held as ``torch.float8_e4m3fn`` values beside fp32 scales: one for
+each 128 columns of a row (activations, ``[M, ceil(K/128)]``) or for each
+128 x 128 tile (weights, ``[N/128, K/128]`` rounded up, with the experts in
+front where there are several).  For a block with largest magnitude ``a`` (at
+least 2**-100) the scale is ``a / 448`` and the values are ``x * (448 / a)``
+rounded to nearest even, so ``q.float() * scale`` stands for ``x``.  A NaN or
+an infinity in a block makes every product over that block NaN.
+
+As in ``bindings``: contiguous CUDA tensors, the current stream of the
+operands' device, ``_into`` forms that return the caller's storage, no
+synchronisation and no autograd.  The products take every K; they run on the
+tensor cores where K is a multiple of 16 and the operands start on 16-byte
+boundaries, elsewhere on a much slower CUDA-core kernel.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .bindings import _call, _ptr, _stream
+
+__all__ = [
+    "quantize_fp8_block128", "quantize_fp8_block128_into",
+    "quantize_fp8_block128_weight", "quantize_fp8_block128_weight_into",
+    "gemm_fp8_block128", "gemm_fp8_block128_into",
+    "gemm_swiglu_fp8_block128", "gemm_swiglu_fp8_block128_into",
+]
+
+BLOCK = 128
+_E4M3 = torch.float8_e4m3fn
+_MAX_SIZE = 0x7FFFFFFF - 1024
+
+
+def _blocks(size: int) -> int:
+    return -(-size // BLOCK)
+
+
+def _check_placement(what: str, *tensors: torch.Tensor) -> None:
+    """Contiguous CUDA tensors of one device."""
+    for t in tensors:
+        if not t.is_contiguous():
+            raise ValueError(f"all {what} tensors must be contiguous")
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError(f"{what} tensors must be CUDA tensors")
+    for t in tensors:
+        if t.device != tensors[0].device:
+            raise ValueError(f"{what} tensors must be on one device")
+
+
+def _check_sizes(what: str, *sizes: int) -> None:
+    for size in sizes:
+        if size > _MAX_SIZE:
+            raise ValueError(f"{what} sizes must be at most {_MAX_SIZE}")
+
+
+def _launch(symbol: str, on: torch.Tensor, *args) -> None:
+    """One library call on the current stream of ``on``'s device."""
+    if on.get_device() == torch.cuda.current_device():
+        _call(symbol, *args, _stream(on))
+    else:
+        with torch.cuda.device(on.device):
+            _call(symbol, *args, _stream(on))
+
+
+# ---------------------------------------------------------------- quantisation
+
+
+def _source_suffix(what: str, x: torch.Tensor) -> str:
+    if x.dtype == torch.bfloat16:
+        return "bf16"
+    if x.dtype == torch.float32:
+        return "f32"
+    raise TypeError(f"{what} expects a bfloat16 or float32 input")
+
+
+def _check_quantized(what: str, x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
+                     scale_shape: tuple[int, ...]) -> None:
+    if q.shape != x.shape:
+        raise ValueError(f"{what} output shape must be {tuple(x.shape)}")
+    if scale.shape != scale_shape:
+        raise ValueError(f"{what} scale shape must be {scale_shape}")
+    if q.dtype != _E4M3 or scale.dtype != torch.float32:
+        raise TypeError(f"{what} writes float8_e4m3fn values and float32 scales")
+
+
+def quantize_fp8_block128_into(x: torch.Tensor, q: torch.Tensor,
+                               scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows [M, K] (bf16 or fp32) to e4m3 [M, K] and fp32 scales [M, ceil(K/128)]."""
+    what = "FP8 quantize"
+    if x.ndim != 2:
+        raise ValueError("x must be 2-D")
+    suffix = _source_suffix(what, x)
+    m, k = x.shape
+    _check_quantized(what, x, q, scale, (m, _blocks(k)))
+    _check_sizes(what, m, k)
+    _check_placement(what, x, q, scale)
+    if m and k:
+        _launch(f"cuda_operator_quantize_fp8_block128_{suffix}", x, _ptr(x), _ptr(q), _ptr(scale),
+                m, k)
+    return q, scale
+
+
+def quantize_fp8_block128(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Allocating form of :func:`quantize_fp8_block128_into`: ``(q, scale)``."""
+    if x.ndim != 2:
+        raise ValueError("x must be 2-D")
+    q = torch.empty(x.shape, device=x.device, dtype=_E4M3)
+    scale = torch.empty((x.shape[0], _blocks(x.shape[1])), device=x.device, dtype=torch.float32)
+    return quantize_fp8_block128_into(x, q, scale)
+
+
+def _weight_scale_shape(shape: torch.Size) -> tuple[int, ...]:
+    return (*shape[:-2], _blocks(shape[-2]), _blocks(shape[-1]))
+
+
+def quantize_fp8_block128_weight_into(weight: torch.Tensor, q: torch.Tensor,
+                                      scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weights [N, K] or [E, N, K] (bf16 or fp32) to e4m3 and fp32 scales of 128 x 128 tiles.
+
+    ``scale`` is [ceil(N/128), ceil(K/128)], with E in front where the weight has it.
+    """
+    what = "FP8 weight quantize"
+    if weight.ndim not in (2, 3):
+        raise ValueError("weight must be 2-D or 3-D")
+    suffix = _source_suffix(what, weight)
+    _check_quantized(what, weight, q, scale, _weight_scale_shape(weight.shape))
+    n, k = weight.shape[-2:]
+    experts = weight.shape[0] if weight.ndim == 3 else 1
+    _check_sizes(what, n, k, experts * _blocks(n) * _blocks(k))
+    _check_placement(what, weight, q, scale)
+    if weight.numel():
+        _launch(f"cuda_operator_quantize_fp8_block128_weight_{suffix}", weight, _ptr(weight),
+                _ptr(q), _ptr(scale), experts, n, k)
+    return q, scale
+
+
+def quantize_fp8_block128_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Allocating form of :func:`quantize_fp8_block128_weight_into`: ``(q, scale)``."""
+    if weight.ndim not in (2, 3):
+        raise ValueError("weight must be 2-D or 3-D")
+    q = torch.empty(weight.shape, device=weight.device, dtype=_E4M3)
+    scale = torch.empty(_weight_scale_shape(weight.shape), device=weight.device,
+                        dtype=torch.float32)
+    return quantize_fp8_block128_weight_into(weight, q, scale)
+
+
+# ---------------------------------------------------------------- products
+
+
+def _check_fp8_operands(what: str, x_fp8: torch.Tensor, x_scale: torch.Tensor,
+                        weight_fp8: torch.Tensor, weight_scale: torch.Tensor,
+                        out: torch.Tensor, swiglu: bool) -> tuple[int, int, int]:
+    """Shapes and types shared by the dense and the grouped products; returns (rows, k, n)."""
+    m, k = x_fp8.shape
+    w_rows = weight_fp8.shape[-2]
+    if weight_fp8.shape[-1] != k:
+        raise ValueError("x.shape[1] must equal the weight's last dimension")
+    if k == 0:
+        raise ValueError(f"{what} requires k > 0")
+    if swiglu and w_rows % (2 * BLOCK):
+        raise ValueError(f"{what} needs gate and up rows in whole blocks of {BLOCK}")
+    n = w_rows // 2 if swiglu else w_rows
+    if x_scale.shape != (m, _blocks(k)):
+        raise ValueError(f"x scale shape must be {(m, _blocks(k))}")
+    if weight_scale.shape != _weight_scale_shape(weight_fp8.shape):
+        raise ValueError(f"weight scale shape must be {_weight_scale_shape(weight_fp8.shape)}")
+    if out.shape != (m, n):
+        raise ValueError(f"output shape must be {(m, n)}")
+    if x_fp8.dtype != _E4M3 or weight_fp8.dtype != _E4M3:
+        raise TypeError(f"{what} expects float8_e4m3fn x and weight")
+    if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+        raise TypeError(f"{what} expects float32 scales")
+    if out.dtype != torch.bfloat16:
+        raise TypeError(f"{what} expects a bfloat16 output")
+    _check_sizes(what, m, k, w_rows)
+    return m, k, n
+
+
+def _gemm_into(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
+               weight_scale: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+    what = "FP8 GEMM SwiGLU" if swiglu else "FP8 GEMM"
+    if x_fp8.ndim != 2 or weight_fp8.ndim != 2:
+        raise ValueError("x and weight must be 2-D")
+    m, k, n = _check_fp8_operands(what, x_fp8, x_scale, weight_fp8, weight_scale, out, swiglu)
+    _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, out)
+    if m and n:
+        symbol = "cuda_operator_gemm_swiglu_fp8_block128" if swiglu else "cuda_operator_gemm_fp8_block128"
+        _launch(symbol, x_fp8, _ptr(x_fp8), _ptr(x_scale), _ptr(weight_fp8), _ptr(weight_scale),
+                _ptr(out), m, k, n)
+    return out
+
+
+def gemm_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
+                           weight_scale: torch.Tensor, out_bf16: torch.Tensor) -> torch.Tensor:
+    """bf16(x @ W.T) of block-scaled e4m3 x [M, K] and W [N, K], products and sums in fp32."""
+    return _gemm_into(False, x_fp8, x_scale, weight_fp8, weight_scale, out_bf16)
+
+
+def gemm_fp8_block128(x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
+                      weight_scale: torch.Tensor) -> torch.Tensor:
+    """Allocating form of :func:`gemm_fp8_block128_into`."""
+    if x_fp8.ndim != 2 or weight_fp8.ndim != 2:
+        raise ValueError("x and weight must be 2-D")
+    out = torch.empty((x_fp8.shape[0], weight_fp8.shape[0]), device=x_fp8.device,
+                      dtype=torch.bfloat16)
+    return gemm_fp8_block128_into(x_fp8, x_scale, weight_fp8, weight_scale, out)
+
+
+def gemm_swiglu_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Tensor,
+                                  packed_weight_fp8: torch.Tensor, weight_scale: torch.Tensor,
+                                  out_bf16: torch.Tensor) -> torch.Tensor:
+    """Packed form: bf16(silu(x @ Wg.T) * (x @ Wu.T)), packed_weight_fp8 [2N, K], gate rows first.
+
+    N must be a multiple of 128, so that no tile of scales spans gate and up rows.
+    """
+    return _gemm_into(True, x_fp8, x_scale, packed_weight_fp8, weight_scale, out_bf16)
+
+
+def gemm_swiglu_fp8_block128(x_fp8: torch.Tensor, x_scale: torch.Tensor,
+                             packed_weight_fp8: torch.Tensor,
+                             weight_scale: torch.Tensor) -> torch.Tensor:
+    """Allocating form of :func:`gemm_swiglu_fp8_block128_into`."""
+    if x_fp8.ndim != 2 or packed_weight_fp8.ndim != 2:
+        raise ValueError("x and weight must be 2-D")
+    out = torch.empty((x_fp8.shape[0], packed_weight_fp8.shape[0] // 2), device=x_fp8.device,
+                      dtype=torch.bfloat16)
+    return gemm_swiglu_fp8_block128_into(x_fp8, x_scale, packed_weight_fp8, weight_scale, out)

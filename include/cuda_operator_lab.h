@@ -287,6 +287,48 @@ int cuda_operator_reduction_partial_f64(const float* input, double* partial, uin
  * looks up the array's device address; make it before any stream capture. */
 int cuda_operator_lab_reduction_noalloc(const float* input, float* output, uint64_t n, void* stream);
 
+/* ---- Expert layers: e4m3 block-128 operands and products grouped by expert --
+ * No reference counterparts; they stand beside the packed GEMM+SwiGLU above.
+ *
+ * e4m3 operands carry one fp32 scale for each block of 128 columns of a row
+ * (activations, scale [m, ceil(k/128)]) or each 128 x 128 tile (weights, scale
+ * [experts, ceil(n/128), ceil(k/128)]):
+ *   a = max(max |x| over the block, 2^-100), scale = a / 448,
+ *   q = e4m3(x * (448 / a)), to nearest even.
+ * A block that holds a NaN or an infinity makes every product over it NaN. */
+int cuda_operator_quantize_fp8_block128_f32(const float* input, void* output_fp8, float* scale, uint64_t m, uint64_t k, void* stream);
+int cuda_operator_quantize_fp8_block128_bf16(const void* input_bf16, void* output_fp8, float* scale, uint64_t m, uint64_t k, void* stream);
+int cuda_operator_quantize_fp8_block128_weight_f32(const float* weight, void* output_fp8, float* scale, uint64_t experts, uint64_t n, uint64_t k, void* stream);
+int cuda_operator_quantize_fp8_block128_weight_bf16(const void* weight_bf16, void* output_fp8, float* scale, uint64_t experts, uint64_t n, uint64_t k, void* stream);
+
+/* out[m, n] = bf16(x . w^T) of e4m3 operands with their scales, products and
+ * sums in fp32.  The swiglu form takes the packed weight [2n, k] (gate rows
+ * first) and gives bf16(silu(gate) * up); it needs n % 128 == 0, so that no
+ * tile of scales spans gate and up rows.  m == 0 or n == 0 succeeds first;
+ * NULL, k == 0 and sizes above INT32_MAX - 1024 are invalid. */
+int cuda_operator_gemm_fp8_block128(const void* input_fp8, const float* input_scale, const void* weight_fp8, const float* weight_scale, void* output_bf16, uint64_t m, uint64_t k, uint64_t n, void* stream);
+int cuda_operator_gemm_swiglu_fp8_block128(const void* input_fp8, const float* input_scale, const void* packed_weight_fp8, const float* weight_scale, void* output_bf16, uint64_t m, uint64_t k, uint64_t n, void* stream);
+
+/* Products grouped by expert: `offsets` (int32 [experts + 1] in device memory,
+ * not decreasing) gives expert e the rows offsets[e] .. offsets[e + 1] of the
+ * t rows of x; weight [experts, n, k] (swiglu: [experts, 2n, k]).  Rows of no
+ * expert (before offsets[0], from offsets[experts] on) are neither used nor
+ * written.  Offsets outside [0, t] are clamped, so no call reads or writes out
+ * of range.  At most 1024 experts; t == 0, n == 0 or experts == 0 succeeds
+ * first, the other rules are those of the dense forms. */
+int cuda_operator_gemm_grouped_bf16(const void* input_bf16, const void* weight_bf16, const int32_t* offsets, void* output_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
+int cuda_operator_gemm_grouped_swiglu_bf16(const void* input_bf16, const void* packed_weight_bf16, const int32_t* offsets, void* output_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
+int cuda_operator_gemm_grouped_fp8_block128(const void* input_fp8, const float* input_scale, const void* weight_fp8, const float* weight_scale, const int32_t* offsets, void* output_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
+int cuda_operator_gemm_grouped_swiglu_fp8_block128(const void* input_fp8, const float* input_scale, const void* packed_weight_fp8, const float* weight_scale, const int32_t* offsets, void* output_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
+
+/* Gradients of cuda_operator_gemm_grouped_bf16, grad [t, n]:
+ *   grad_input[r, :]     = sum_j grad[r, j] weight[e, j, :]   (r a row of e)
+ *   grad_weight[e, j, :] = sum_r grad[r, j] input[r, :]       (r the rows of e)
+ * bf16 in and out, fp32 sums in a fixed order.  grad_weight is written for
+ * every expert, zeros where it has no rows (t == 0 included). */
+int cuda_operator_gemm_grouped_bf16_grad_input(const void* grad_bf16, const void* weight_bf16, const int32_t* offsets, void* grad_input_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
+int cuda_operator_gemm_grouped_bf16_grad_weight(const void* grad_bf16, const void* input_bf16, const int32_t* offsets, void* grad_weight_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
+
 /* Number of SMs of the current device and the library's build tag; lets a
  * caller check which library it loaded.  Host-only, enqueues nothing. */
 int cuda_operator_lab_device_info(int* sm_count, int* cc_major, int* cc_minor);
