@@ -1,10 +1,21 @@
 // Products grouped by expert (bf16, both gradients, block-scaled e4m3) and the
 // dense block-scaled e4m3 products, which are the same with a single group.
+#include <atomic>
+#include <cstdlib>
+#include <cstring>
+
 #include "gemm_grouped_simt.cuh"
+#include "gemm_grouped_sm100.cuh"
+#include "gemm_host.cuh"
 
 namespace {
 
 using col::simt::GroupedSimtParams;
+using col::sm100::GroupedCfg;
+using col::sm100::GroupedParams;
+using col::sm100::kForward;
+using col::sm100::kGradW;
+using col::sm100::kGradX;
 
 constexpr std::uint64_t kIntMax = 0x7fffffffull;
 
@@ -32,6 +43,172 @@ GroupedSimtParams simt_params(const void* a, const void* b, const std::int32_t* 
   return p;
 }
 
+// ---------------------------------------------------------------- tensor maps
+
+// A tensor map is a pure function of these; the calling thread keeps the last
+// few, since a call on the same weights or reused buffers needs the same map
+// (as gemm.cu does for the dense products).
+struct MapKey {
+  const void* base;
+  std::uint64_t cols;     // contiguous elements
+  std::uint64_t rows;
+  std::uint64_t experts;  // 0: two-dimensional
+  std::uint32_t box_rows;
+  std::uint32_t elem;     // bytes
+};
+
+// Map over row-major [experts][rows][cols]; box = 128 bytes of columns (the
+// swizzle span) x box_rows rows.  Out-of-range boxes read zeros.
+int encode_map(CUtensorMap* map, const MapKey& key) {
+  struct Entry {
+    CUtensorMap map;
+    MapKey key;
+    bool valid;
+  };
+  constexpr int kEntries = 32;
+  thread_local Entry cache[kEntries] = {};
+  const std::uintptr_t h = (reinterpret_cast<std::uintptr_t>(key.base) >> 7) ^ (key.rows * 31u) ^
+                           (key.cols * 131u) ^ (key.experts * 7u) ^
+                           (static_cast<std::uintptr_t>(key.box_rows) * 13u);
+  Entry& e = cache[(h ^ (h >> 5) ^ (h >> 10)) % kEntries];
+  if (e.valid && e.key.base == key.base && e.key.cols == key.cols && e.key.rows == key.rows &&
+      e.key.experts == key.experts && e.key.box_rows == key.box_rows && e.key.elem == key.elem) {
+    std::memcpy(map, &e.map, sizeof(CUtensorMap));
+    return 0;
+  }
+  auto enc = col::tensor_map_encoder();
+  if (!enc) return col::kErrNoTensorMapEncoder;
+  const cuuint64_t dims[3] = {key.cols, key.rows, key.experts};
+  const cuuint64_t strides[2] = {key.cols * key.elem, key.cols * key.rows * key.elem};
+  const cuuint32_t box[3] = {128 / key.elem, key.box_rows, 1};
+  const cuuint32_t estrides[3] = {1, 1, 1};
+  const CUresult r = enc(
+      map, key.elem == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8,
+      key.experts == 0 ? 2 : 3, const_cast<void*>(key.base), dims, strides, box, estrides,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return col::kErrTensorMapEncode;
+  std::memcpy(&e.map, map, sizeof(CUtensorMap));
+  e.key = key;
+  e.valid = true;
+  return 0;
+}
+
+// Whether TMA can address rows of `cols` elements from `base`.
+inline bool tma_ok(const void* base, std::uint64_t cols, std::uint32_t elem) {
+  return col::aligned16(base) && (cols * elem) % 16 == 0;
+}
+
+// ---------------------------------------------------------------- launches
+
+// Dynamic shared memory of a kernel, set once per device.
+template <typename Kernel>
+int allow_smem(Kernel kernel, std::uint32_t bytes, int dev, std::atomic<std::uint64_t>& done) {
+  const std::uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return 0;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(bytes));
+  if (e != cudaSuccess) return static_cast<int>(e);
+  done.fetch_or(bit, std::memory_order_release);
+  return 0;
+}
+
+// Workers (CTAs or CTA pairs) that can be resident at once.
+template <typename Kernel>
+int resident_pairs(Kernel kernel, std::uint32_t smem, int dev) {
+  static std::atomic<int> cached[64] = {};
+  int pairs = cached[dev & 63].load(std::memory_order_acquire);
+  if (pairs != 0) return pairs;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2, 1, 1);
+  cfg.blockDim = dim3(col::sm100::kCtaThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&pairs, kernel, &cfg) != cudaSuccess || pairs <= 0) {
+    cudaGetLastError();
+    pairs = -1;
+  }
+  cached[dev & 63].store(pairs, std::memory_order_release);
+  return pairs;
+}
+
+template <int MODE, bool SWIGLU, int CG, int BN>
+int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int sm_count,
+                        cudaStream_t s) {
+  using Cfg = GroupedCfg<CG, BN>;
+  auto kernel = col::sm100::grouped_bf16_kernel<MODE, SWIGLU, CG, BN>;
+  static std::atomic<std::uint64_t> done{0};
+  if (int rc = allow_smem(kernel, Cfg::kSmemBytes, dev, done)) return rc;
+  int workers = sm_count;
+  if constexpr (CG == 2) {
+    workers = resident_pairs(kernel, Cfg::kSmemBytes, dev);
+    if (workers <= 0) return static_cast<int>(cudaErrorInvalidConfiguration);
+  }
+  if (most_tiles < static_cast<std::uint64_t>(workers)) workers = static_cast<int>(most_tiles);
+  return col::launch_serialised(kernel, dim3(static_cast<unsigned>(workers * CG)),
+                                dim3(col::sm100::kCtaThreads), Cfg::kSmemBytes, s, p);
+}
+
+// Tensor-core product; -1 where TMA cannot address the operands.
+template <int MODE, bool SWIGLU>
+int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, void* out,
+                    std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
+                    cudaStream_t s) {
+  const std::uint64_t w_rows = SWIGLU ? 2 * n : n;
+  const std::uint64_t a_cols = MODE == kForward ? k : n;
+  if (!tma_ok(a, a_cols, 2) || !tma_ok(b, k, 2)) return -1;
+  int dev = 0;
+  const col::DeviceInfo& info = col::device_info(&dev);
+  if (info.cc_major != 10) return col::kErrDeviceNotSupported;
+  GroupedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.status = col::gemm_status_ptr(dev);
+  if (!p.status) return static_cast<int>(cudaErrorInvalidDevice);
+  const std::uint64_t out_cols = MODE == kForward ? n : k;
+  p.offsets = offsets;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.rows = static_cast<int>(t);
+  p.groups = static_cast<int>(experts);
+  p.out_cols = static_cast<int>(out_cols);
+  p.out_rows = static_cast<int>(n);
+  p.num_k_blocks = static_cast<int>(((MODE == kForward ? k : n) + 63) / 64);
+  p.up_offset = static_cast<int>(n);
+  p.out_vec_ok = col::aligned16(out) && out_cols % 8 == 0;
+
+  int cg = t >= 256 * experts ? 2 : 1;
+  int bn = cg == 2 ? 256 : 128;
+  if (const char* force = std::getenv("GROUPED_VARIANT")) {
+    cg = force[0] - '0';
+    bn = std::atoi(force + 1);
+  }
+  p.num_n_blocks = static_cast<int>((out_cols * (SWIGLU ? 2 : 1) + bn - 1) / bn);
+  const std::uint64_t m_tiles = MODE == kGradW ? experts * ((n + 128 * cg - 1) / (128 * cg))
+                                               : t / (128 * cg) + experts;
+  const std::uint64_t most_tiles = m_tiles * p.num_n_blocks;
+  if (most_tiles > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
+  const std::uint32_t a_box = MODE == kGradW ? 64 : (cg == 1 ? 32 : 128);
+  const std::uint32_t b_box = MODE == kForward ? bn / 2 : 64;
+  int rc = encode_map(&p.map_a, {a, a_cols, t, 0, a_box, 2});
+  if (rc == 0) {
+    rc = MODE == kGradW ? encode_map(&p.map_b, {b, k, t, 0, b_box, 2})
+                        : encode_map(&p.map_b, {b, k, w_rows, experts, b_box, 2});
+  }
+  if (rc != 0) return rc;
+  if (cg == 2) {
+    if (bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 2, 256>(p, most_tiles, dev, info.sm_count, s);
+    return launch_grouped_bf16<MODE, SWIGLU, 2, 128>(p, most_tiles, dev, info.sm_count, s);
+  }
+  if (bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 1, 256>(p, most_tiles, dev, info.sm_count, s);
+  if (bn == 128) return launch_grouped_bf16<MODE, SWIGLU, 1, 128>(p, most_tiles, dev, info.sm_count, s);
+  return launch_grouped_bf16<MODE, SWIGLU, 1, 64>(p, most_tiles, dev, info.sm_count, s);
+}
+
 template <bool SWIGLU>
 int grouped_forward_bf16(const void* x, const void* w, const std::int32_t* offsets, void* out,
                          std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
@@ -41,9 +218,11 @@ int grouped_forward_bf16(const void* x, const void* w, const std::int32_t* offse
   if (!x || !w || !offsets || !out || !sizes_ok(t, k, n, experts) || w_rows > kIntMax - 1024) {
     return static_cast<int>(cudaErrorInvalidValue);
   }
+  const cudaStream_t s = col::as_stream(stream);
+  const int rc = grouped_bf16_tc<kForward, SWIGLU>(x, w, offsets, out, t, k, n, experts, s);
+  if (rc != -1) return rc;
   const GroupedSimtParams p = simt_params(x, w, offsets, out, t, k, n, w_rows, experts);
-  return col::simt::launch_grouped_simt<__nv_bfloat16, col::simt::kForward, SWIGLU>(
-      p, col::as_stream(stream));
+  return col::simt::launch_grouped_simt<__nv_bfloat16, col::simt::kForward, SWIGLU>(p, s);
 }
 
 template <bool SWIGLU>
@@ -93,10 +272,13 @@ COL_API int cuda_operator_gemm_grouped_bf16_grad_input(const void* grad_bf16,
       !sizes_ok(t, k, n, experts)) {
     return static_cast<int>(cudaErrorInvalidValue);
   }
+  const cudaStream_t s = col::as_stream(stream);
+  const int rc = grouped_bf16_tc<kGradX, false>(grad_bf16, weight_bf16, offsets, grad_input_bf16, t,
+                                                k, n, experts, s);
+  if (rc != -1) return rc;
   const GroupedSimtParams p =
       simt_params(grad_bf16, weight_bf16, offsets, grad_input_bf16, t, k, n, n, experts);
-  return col::simt::launch_grouped_simt<__nv_bfloat16, col::simt::kGradX, false>(
-      p, col::as_stream(stream));
+  return col::simt::launch_grouped_simt<__nv_bfloat16, col::simt::kGradX, false>(p, s);
 }
 
 COL_API int cuda_operator_gemm_grouped_bf16_grad_weight(const void* grad_bf16,
@@ -110,10 +292,17 @@ COL_API int cuda_operator_gemm_grouped_bf16_grad_weight(const void* grad_bf16,
       !sizes_ok(t, k, n, experts)) {
     return static_cast<int>(cudaErrorInvalidValue);
   }
+  const cudaStream_t s = col::as_stream(stream);
+  int rc = -1;
+  if (t != 0) {
+    rc = grouped_bf16_tc<kGradW, false>(grad_bf16, input_bf16, offsets, grad_weight_bf16, t, k, n,
+                                        experts, s);
+  }
+  if (rc != -1) return rc;
+  // also t == 0 (there is nothing to address): every sum is empty, all zeros
   const GroupedSimtParams p =
       simt_params(grad_bf16, input_bf16, offsets, grad_weight_bf16, t, k, n, n, experts);
-  return col::simt::launch_grouped_simt<__nv_bfloat16, col::simt::kGradW, false>(
-      p, col::as_stream(stream));
+  return col::simt::launch_grouped_simt<__nv_bfloat16, col::simt::kGradW, false>(p, s);
 }
 
 COL_API int cuda_operator_gemm_fp8_block128(const void* input_fp8, const float* input_scale,

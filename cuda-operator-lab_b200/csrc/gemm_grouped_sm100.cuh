@@ -1,0 +1,572 @@
+// Tensor-core (tcgen05) products grouped by expert: bf16 operands, fp32 sums.
+//
+// For the rows r of group g (grouped_schedule.cuh):
+//   kForward  out[r, j]   = sum_c x[r, c] w[g, j, c]        (SwiGLU: silu(gate) * up)
+//   kGradX    dx[r, c]    = sum_j dy[r, j] w[g, j, c]
+//   kGradW    dw[g, j, c] = sum_r dy[r, j] x[r, c]
+//
+// Persistent and warp-specialised like the dense kernel (gemm_sm100.cuh):
+// warp 0 loads, warp 1 issues the MMAs, warp 2 owns TMEM, warp 3 builds the
+// table of row tiles and zeroes ragged tails (kGradW), warps 4..11 store.  CG =
+// 1: a CTA computes 128 rows; CG = 2: a pair of CTAs computes 256 rows, each
+// holding half of B (tcgen05 cta_group::2).  BN accumulator columns a tile, two
+// accumulators in TMEM, so that storing a tile overlaps the next one's MMAs.
+//
+// Every operand is read in place.  Forward reads A and B along the summed
+// index (K-major).  The gradients sum over an index that is not the
+// contiguous one: w in kGradX and both operands in kGradW are loaded as boxes
+// of 64 contiguous columns x 64 summed rows and multiplied as MN-major tiles,
+// so nothing is transposed in memory.
+//
+// Ragged edges: a tile that reaches past its group's last row loads rows of
+// the next group, which only reach accumulator rows that are not stored.  In
+// kGradW the rows are summed over, so the last block of a group is cut to
+// whole steps of 16 rows and the rest of its last step is set to zero in shared
+// memory, in both operands (a NaN there times zero would be a NaN).  Edges of
+// n and k are filled with zeros by TMA; w is a three-dimensional map, so that a
+// box never runs into the next expert.
+#pragma once
+
+#include "gemm_sm100.cuh"
+#include "gemm_sm100_2sm.cuh"
+#include "grouped_schedule.cuh"
+
+namespace col {
+namespace sm100 {
+
+enum GroupedMode : int { kForward = 0, kGradX = 1, kGradW = 2 };
+
+struct __align__(64) GroupedParams {
+  CUtensorMap map_a;
+  CUtensorMap map_b;
+  const int* offsets;
+  __nv_bfloat16* out;
+  unsigned* status;
+  int rows;          // t
+  int groups;
+  int out_cols;      // n (kForward), k (gradients)
+  int out_rows;      // kGradW: n
+  int num_n_blocks;  // tiles along out_cols
+  int num_k_blocks;  // blocks of the summed index (kGradW: by group)
+  int up_offset;     // SwiGLU: rows from gate to up in w
+  int out_vec_ok;    // 16-byte stores allowed
+};
+
+constexpr uint32_t kGroupedTableBytes = 4352;  // prefix table of kMaxGroups + 1 ints
+static_assert(kGroupedTableBytes >= (kMaxGroups + 1) * 4, "table size");
+
+template <int CG, int BN>
+struct GroupedCfg {
+  static_assert(BN == 64 || BN == 128 || BN == 256, "tile width");
+  static_assert(CG == 1 || CG == 2, "CTAs of a tile");
+  static constexpr int kTileRows = kBlockM * CG;
+  static constexpr uint32_t kABytes = kBlockM * kBlockK * 2;
+  static constexpr uint32_t kBBytes = BN / CG * kBlockK * 2;
+  static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
+  static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : 2;  // k-blocks a stage
+  static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
+  static constexpr uint32_t kExtraBytes = 256 + kGroupedTableBytes;
+  static constexpr int kStagesFit =
+      static_cast<int>((kSmemLimit - 1024 - kExtraBytes) / kStageBytes);
+  static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
+  static constexpr uint32_t kTmemCols = 2 * BN;
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024 + kExtraBytes;
+};
+
+// MN-major tile with the 128-byte swizzle: chunks of 64 contiguous elements,
+// `chunk_bytes` apart (leading offset), rows of the summed index 128 bytes
+// apart in groups of 8 (stride offset 1024).  A step of 16 rows is 2048 bytes.
+__device__ __forceinline__ uint64_t sdesc_mnmajor_sw128(uint32_t saddr, uint32_t chunk_bytes) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) |
+         (static_cast<uint64_t>(chunk_bytes >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+         (static_cast<uint64_t>(2) << 61);
+}
+
+constexpr uint32_t kIdescAMnMajor = 1u << 15;
+constexpr uint32_t kIdescBMnMajor = 1u << 16;
+
+template <int CG>
+__device__ __forceinline__ void grouped_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                                int x, int y) {
+  if constexpr (CG == 2) {
+    tma_load_2d_pair(dst, map, bar, x, y);
+  } else {
+    tma_load_2d(dst, map, bar, x, y);
+  }
+}
+
+template <int CG>
+__device__ __forceinline__ void grouped_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                                int x, int y, int z) {
+  if constexpr (CG == 2) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+  }
+}
+
+// All MMAs issued so far by this thread: arrive on `bar` (both CTAs of a pair).
+template <int CG>
+__device__ __forceinline__ void grouped_commit(uint32_t bar) {
+  if constexpr (CG == 2) {
+    umma_commit_pair_both(bar);
+  } else {
+    umma_commit(bar);
+  }
+}
+
+// What the roles share about one tile.
+struct GroupedTile {
+  int group;
+  int a_row;    // first row of this CTA's half of the tile (kGradW: of n)
+  int col;      // first output column
+  int begin;    // the group's rows
+  int end;
+  int k_blocks;
+};
+
+template <int MODE, bool SWIGLU, int CG, int BN>
+__device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, const int* prefix,
+                                                    int tile, int rank) {
+  using Cfg = GroupedCfg<CG, BN>;
+  GroupedTile t;
+  TileCoords c;
+  if constexpr (MODE == kGradW) {
+    // every group has the same tiles
+    const int m_blocks = (p.out_rows + Cfg::kTileRows - 1) / Cfg::kTileRows;
+    const int per_group = m_blocks * p.num_n_blocks;
+    c.group = tile / per_group;
+    const int local = tile - c.group * per_group;
+    c.m = local % m_blocks;
+    c.n = local / m_blocks;
+  } else {
+    c = tile_of(tile, prefix, p.groups, p.num_n_blocks);
+  }
+  const RowRange r = group_rows(p.offsets, c.group, p.rows);
+  t.group = c.group;
+  t.begin = r.begin;
+  t.end = r.end;
+  t.a_row = (MODE == kGradW ? 0 : r.begin) + c.m * Cfg::kTileRows + rank * kBlockM;
+  t.col = c.n * (SWIGLU ? BN / 2 : BN);
+  t.k_blocks = MODE == kGradW ? (r.end - r.begin + kBlockK - 1) / kBlockK : p.num_k_blocks;
+  return t;
+}
+
+// Rows of the summed index in the last block of a kGradW tile; 0: it is whole
+// steps of 16 and needs no zeroing.
+__device__ __forceinline__ int ragged_rows(const GroupedTile& t) {
+  const int last = (t.end - t.begin) % kBlockK;
+  return last % 16 == 0 ? 0 : last;
+}
+
+// One row of W consecutive outputs.
+template <int W>
+__device__ __forceinline__ void grouped_store(const GroupedParams& p, std::size_t row, int col0,
+                                              const float (&o)[W]) {
+  __nv_bfloat16* dst = p.out + row * p.out_cols + col0;
+  if (p.out_vec_ok && col0 + W <= p.out_cols) {
+    uint4* d4 = reinterpret_cast<uint4*>(dst);
+#pragma unroll
+    for (int j = 0; j < W / 8; ++j) {
+      d4[j] = make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]),
+                         pack_bf16x2(o[8 * j + 4], o[8 * j + 5]),
+                         pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      if (col0 + j < p.out_cols) dst[j] = __float2bfloat16_rn(o[j]);
+    }
+  }
+}
+
+template <int MODE, bool SWIGLU, int CG, int BN>
+__global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
+    grouped_bf16_kernel(const __grid_constant__ GroupedParams p) {
+  using Cfg = GroupedCfg<CG, BN>;
+  static_assert(MODE == kForward || !SWIGLU, "SwiGLU is a forward epilogue");
+  constexpr int kStages = Cfg::kStages;
+  constexpr int kKps = Cfg::kKps;
+  constexpr uint32_t kIdesc = idesc_bf16_f32(Cfg::kTileRows, BN) |
+                              (MODE == kGradW ? kIdescAMnMajor : 0u) |
+                              (MODE != kForward ? kIdescBMnMajor : 0u);
+  constexpr uint32_t kChunkBytes = 64 * kBlockK * 2;  // 64 columns x 64 rows
+  // Forward with single CTAs serves few rows a group: A is loaded 32 rows at a
+  // time, only those the group has.
+  constexpr int kABoxRows = MODE == kGradW ? kBlockK : (CG == 1 ? 32 : kBlockM);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<std::uintptr_t>(smem_raw) + 1023) & ~static_cast<std::uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * Cfg::kStageBytes);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + kStages;
+  uint64_t* tfull_bar = bars + 2 * kStages;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint64_t* tail_bar = drain_bar + 1;  // kStages of them
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tail_bar + kStages);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  static_assert((3 * kStages + 5) * 8 + 8 <= 256, "barrier space");
+  int* prefix = reinterpret_cast<int*>(smem + kStages * Cfg::kStageBytes + 256);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
+  const bool leader = rank == 0;
+  const int worker = blockIdx.x / CG;
+  const int workers = gridDim.x / CG;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      // kGradW pairs: both CTAs arrive for a stage (see the tail below)
+      mbar_init(smem_u32(full_bar + s), MODE == kGradW ? CG : 1);
+      mbar_init(smem_u32(empty_bar + s), 1);
+      mbar_init(smem_u32(tail_bar + s), 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(smem_u32(tfull_bar + a), 1);
+      mbar_init(smem_u32(tempty_bar + a), CG * kEpiWarps);
+    }
+    mbar_init(smem_u32(drain_bar), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    grid_dependents_launch();
+  }
+  if (warp == 2) {
+    if constexpr (CG == 2) {
+      tmem_alloc_pair(smem_u32(tmem_holder), Cfg::kTmemCols);
+    } else {
+      tmem_alloc(smem_u32(tmem_holder), Cfg::kTmemCols);
+    }
+  }
+  // The offsets may come from the kernel before this one.
+  grid_dependency_wait();
+  if (MODE != kGradW && warp == 3) {
+    fill_tile_prefix(prefix, p.offsets, p.groups, p.rows, Cfg::kTileRows, lane);
+  }
+  tc_fence_before();
+  if constexpr (CG == 2) {
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  auto fail = [&](unsigned code) {
+    atomicOr(p.status, code);
+    *abort_flag = 1;
+  };
+  int num_tiles;
+  if constexpr (MODE == kGradW) {
+    num_tiles = p.groups * ((p.out_rows + Cfg::kTileRows - 1) / Cfg::kTileRows) * p.num_n_blocks;
+  } else {
+    num_tiles = prefix[p.groups] * p.num_n_blocks;
+  }
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---------------- TMA producer
+      prefetch_tmap(&p.map_a);
+      prefetch_tmap(&p.map_b);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t issued_mask = 0;
+      uint32_t issued_phase = 0;
+      int filled = 0;
+      bool ok = true;
+      for (int tile = worker; ok && tile < num_tiles; tile += workers) {
+        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
+        int a_boxes = kBlockM / kABoxRows;
+        if constexpr (MODE != kGradW && CG == 1) {
+          a_boxes = min(a_boxes, (t.end - t.a_row + kABoxRows - 1) / kABoxRows);
+        }
+        const bool ragged = MODE == kGradW && ragged_rows(t) != 0;
+        for (int kb = 0; kb < t.k_blocks; kb += kKps) {
+          if (filled >= kStages && !mbar_wait(smem_u32(empty_bar + stage), phase ^ 1u, abort_flag)) {
+            fail(kStatusProducer);
+            ok = false;
+            break;
+          }
+          const int nk = min(kKps, t.k_blocks - kb);
+          const uint32_t a_bytes =
+              MODE != kGradW && CG == 1 ? a_boxes * kABoxRows * 128u : Cfg::kABytes;
+          const uint32_t bytes = nk * (a_bytes + Cfg::kBBytes);
+          const uint32_t fb_local = smem_u32(full_bar + stage);
+          uint32_t fb = fb_local;
+          if constexpr (CG == 2) fb = map_to_cta(fb_local, 0);
+          if (ragged && kb + nk == t.k_blocks) {
+            // A tail that needs zeroing completes on this CTA's own barrier;
+            // the zeroing warp then arrives on the stage's.
+            fb = smem_u32(tail_bar + stage);
+            mbar_arrive_expect_tx(fb, bytes);
+            if constexpr (CG == 2) fb = map_to_cta(fb, rank);
+          } else if (leader) {
+            mbar_arrive_expect_tx(fb_local, CG * bytes);
+          } else if constexpr (MODE == kGradW) {
+            mbar_arrive_cluster(fb);
+          }
+#pragma unroll
+          for (int j = 0; j < kKps; ++j) {
+            if (j >= nk) break;
+            const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
+            const uint32_t sb = sa + Cfg::kABytes;
+            const int kc = (kb + j) * kBlockK;
+            if constexpr (MODE == kGradW) {
+#pragma unroll
+              for (int i = 0; i < kBlockM / 64; ++i) {
+                grouped_load_2d<CG>(sa + i * kChunkBytes, &p.map_a, fb, t.a_row + 64 * i,
+                                    t.begin + kc);
+              }
+            } else {
+              for (int i = 0; i < a_boxes; ++i) {
+                grouped_load_2d<CG>(sa + i * (kABoxRows * 128), &p.map_a, fb, kc,
+                                    t.a_row + i * kABoxRows);
+              }
+            }
+            if constexpr (MODE == kForward) {
+              // half h of B: rows n0 + h BN/2 of w, or gate (0) and up (1) rows
+#pragma unroll
+              for (int i = 0; i < 2 / CG; ++i) {
+                const int h = CG == 2 ? rank : i;
+                grouped_load_3d<CG>(sb + i * (BN / 2 * 128), &p.map_b, fb, kc,
+                                    t.col + h * (SWIGLU ? p.up_offset : BN / 2), t.group);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < BN / CG / 64; ++i) {
+                const int col = t.col + rank * (BN / CG) + 64 * i;
+                if constexpr (MODE == kGradX) {
+                  grouped_load_3d<CG>(sb + i * kChunkBytes, &p.map_b, fb, col, kc, t.group);
+                } else {
+                  grouped_load_2d<CG>(sb + i * kChunkBytes, &p.map_b, fb, col, t.begin + kc);
+                }
+              }
+            }
+          }
+          if (filled < kStages) ++filled;
+          issued_mask |= 1u << stage;
+          issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      if (!ok || *abort_flag) {
+        if (leader) {
+          for (int s = 0; s < kStages; ++s) {
+            if ((issued_mask & (1u << s)) &&
+                !mbar_wait_drain(smem_u32(full_bar + s), (issued_phase >> s) & 1u)) {
+              atomicOr(p.status, kStatusDrain);
+            }
+          }
+        } else {
+          // CTA 1 cannot observe CTA 0's barriers: give its copies time to land.
+          for (int i = 0; i < 200; ++i) __nanosleep(1000);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      // ---------------- MMA issuer
+      int stage = 0;
+      uint32_t phase = 0;
+      int local = 0;
+      bool ok = true;
+      bool issued_any = false;
+      for (int tile = worker; ok && tile < num_tiles; tile += workers) {
+        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
+        if (MODE == kGradW && t.k_blocks == 0) continue;  // zeros, stored without a sum
+        const int acc = local & 1;
+        if (!mbar_wait(smem_u32(tempty_bar + acc), ((local >> 1) & 1) ^ 1u, abort_flag)) {
+          fail(kStatusMma);
+          break;
+        }
+        ++local;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        const int last_rows = MODE == kGradW ? t.end - t.begin - (t.k_blocks - 1) * kBlockK : 0;
+        for (int kb = 0; kb < t.k_blocks; kb += kKps) {
+          if (!mbar_wait(smem_u32(full_bar + stage), phase, abort_flag)) {
+            fail(kStatusMma);
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int nk = min(kKps, t.k_blocks - kb);
+#pragma unroll
+          for (int j = 0; j < kKps; ++j) {
+            if (j >= nk) break;
+            const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
+            const uint32_t sb = sa + Cfg::kABytes;
+            int steps = kBlockK / 16;
+            if (MODE == kGradW && kb + j == t.k_blocks - 1) steps = (last_rows + 15) / 16;
+#pragma unroll
+            for (int k = 0; k < kBlockK / 16; ++k) {
+              if (MODE == kGradW && k >= steps) break;
+              const uint64_t ad = MODE == kGradW ? sdesc_mnmajor_sw128(sa + k * 2048, kChunkBytes)
+                                                 : sdesc_kmajor_sw128(sa + k * 32);
+              const uint64_t bd = MODE == kForward ? sdesc_kmajor_sw128(sb + k * 32)
+                                                   : sdesc_mnmajor_sw128(sb + k * 2048, kChunkBytes);
+              const uint32_t accumulate = (kb + j != 0 || k != 0) ? 1u : 0u;
+              if constexpr (CG == 2) {
+                umma_bf16_pair(d_tmem, ad, bd, kIdesc, accumulate);
+              } else {
+                umma_bf16(d_tmem, ad, bd, kIdesc, accumulate);
+              }
+            }
+          }
+          issued_any = true;
+          grouped_commit<CG>(smem_u32(empty_bar + stage));
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        grouped_commit<CG>(smem_u32(tfull_bar + acc));
+      }
+      if (issued_any) {
+        if constexpr (CG == 2) {
+          umma_commit_pair_local(smem_u32(drain_bar));
+        } else {
+          umma_commit(smem_u32(drain_bar));
+        }
+        if (!mbar_wait_drain(smem_u32(drain_bar), 0)) atomicOr(p.status, kStatusDrain);
+      }
+    }
+  } else if (warp == 3) {
+    if constexpr (MODE == kGradW) {
+      // ---------------- zeroes the rows behind a group's last one
+      int stage = 0;  // slot of this tile's first stage
+      uint32_t tail_phase = 0;  // bit s: parity of tail_bar[s]'s next completion
+      for (int tile = worker; tile < num_tiles; tile += workers) {
+        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
+        const int stages = (t.k_blocks + kKps - 1) / kKps;
+        const int first = ragged_rows(t);
+        if (first != 0) {
+          const int slot = (stage + stages - 1) % kStages;
+          const bool got =
+              mbar_wait(smem_u32(tail_bar + slot), (tail_phase >> slot) & 1u, abort_flag);
+          tail_phase ^= 1u << slot;
+          if (!got) {
+            if (lane == 0) fail(kStatusProducer);
+            break;
+          }
+          const int j = (t.k_blocks - 1) % kKps;
+          uint8_t* block = smem + slot * Cfg::kStageBytes + j * Cfg::kKBlockBytes;
+          const int count = ((first + 15) / 16 * 16 - first) * 8;  // 16-byte pieces a chunk
+          constexpr int kChunks = static_cast<int>(Cfg::kKBlockBytes / kChunkBytes);
+#pragma unroll 1
+          for (int c = 0; c < kChunks; ++c) {
+            uint4* rows = reinterpret_cast<uint4*>(block + c * kChunkBytes + first * 128);
+            for (int i = lane; i < count; i += 32) rows[i] = make_uint4(0u, 0u, 0u, 0u);
+          }
+          // the MMAs read these rows through the async proxy
+          asm volatile("fence.proxy.async;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            const uint32_t fb = smem_u32(full_bar + slot);
+            if constexpr (CG == 2) {
+              mbar_arrive_cluster(map_to_cta(fb, 0));
+            } else {
+              mbar_arrive(fb);
+            }
+          }
+          __syncwarp();
+        }
+        stage = (stage + stages) % kStages;
+      }
+    }
+  } else if (warp >= 4) {
+    // ---------------- epilogue: this CTA's 128 rows of the tile
+    const int q = warp & 3;
+    const int half = (warp - 4) >> 2;
+    int local = 0;
+    for (int tile = worker; tile < num_tiles; tile += workers) {
+      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
+      const int row = t.a_row + q * 32 + lane;
+      const bool row_ok = row < (MODE == kGradW ? p.out_rows : t.end);
+      const std::size_t out_row =
+          MODE == kGradW ? static_cast<std::size_t>(t.group) * p.out_rows + row : row;
+      if (MODE == kGradW && t.k_blocks == 0) {
+        const float zero[16] = {};
+        for (int c = half * 16; c < BN; c += 32) {
+          if (row_ok) grouped_store<16>(p, out_row, t.col + c, zero);
+        }
+        continue;
+      }
+      const int acc = local & 1;
+      if (!epi_wait(smem_u32(tfull_bar + acc), (local >> 1) & 1, abort_flag, lane)) {
+        if (lane == 0) fail(kStatusEpilogue);
+        break;
+      }
+      ++local;
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
+      // a warp whose rows all lie behind the group's last has nothing to store
+      if (__any_sync(0xffffffffu, row_ok)) {
+        if constexpr (SWIGLU) {
+#pragma unroll 1
+          for (int c = half * 16; c < BN / 2; c += 32) {
+            uint32_t g[16], u[16];
+            tmem_ld16x2(t_row + c, t_row + BN / 2 + c, g, u);
+            float o[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = silu_fast(__uint_as_float(g[j])) * __uint_as_float(u[j]);
+            if (row_ok) grouped_store<16>(p, out_row, t.col + c, o);
+          }
+        } else {
+#pragma unroll 1
+          for (int c = half * 32; c < BN; c += 64) {
+            uint32_t a[32];
+            tmem_ld32(t_row + c, a);
+            float o[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(a[j]);
+            if (row_ok) grouped_store<32>(p, out_row, t.col + c, o);
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CG == 2) {
+          mbar_arrive_cluster(map_to_cta(smem_u32(tempty_bar + acc), 0));
+        } else {
+          mbar_arrive(smem_u32(tempty_bar + acc));
+        }
+      }
+    }
+  }
+
+  // No CTA leaves while its partner may still address its shared memory.
+  __syncwarp();
+  tc_fence_before();
+  if constexpr (CG == 2) {
+    cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  if (warp == 2) {
+    tc_fence_after();
+    if constexpr (CG == 2) {
+      tmem_dealloc_pair(tmem_base, Cfg::kTmemCols);
+    } else {
+      tmem_dealloc(tmem_base, Cfg::kTmemCols);
+    }
+  }
+}
+
+}  // namespace sm100
+}  // namespace col
