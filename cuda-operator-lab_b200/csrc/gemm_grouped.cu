@@ -4,6 +4,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "gemm_fp8_sm100.cuh"
 #include "gemm_grouped_simt.cuh"
 #include "gemm_grouped_sm100.cuh"
 #include "gemm_host.cuh"
@@ -209,6 +210,80 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   return launch_grouped_bf16<MODE, SWIGLU, 1, 64>(p, most_tiles, dev, info.sm_count, s);
 }
 
+template <bool SWIGLU, int CG, int BN>
+int launch_fp8(col::sm100::Fp8Params& p, std::uint64_t most_tiles, int dev, int sm_count,
+               cudaStream_t s) {
+  using Cfg = col::sm100::Fp8Cfg<CG, BN>;
+  auto kernel = col::sm100::fp8_kernel<SWIGLU, CG, BN>;
+  static std::atomic<std::uint64_t> done{0};
+  if (int rc = allow_smem(kernel, Cfg::kSmemBytes, dev, done)) return rc;
+  if constexpr (col::sm100::fp8_split_regs(BN)) {
+    // The warps that take registers over wait until they are free, so the
+    // kernel must have been compiled to start with enough of them.
+    static const bool covered = [kernel]() {
+      cudaFuncAttributes attr;
+      return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess &&
+             attr.numRegs >= col::sm100::kRegsLaunchNeeded;
+    }();
+    if (!covered) return static_cast<int>(cudaErrorInvalidConfiguration);
+  }
+  int workers = sm_count;
+  if constexpr (CG == 2) {
+    workers = resident_pairs(kernel, Cfg::kSmemBytes, dev);
+    if (workers <= 0) return static_cast<int>(cudaErrorInvalidConfiguration);
+  }
+  if (most_tiles < static_cast<std::uint64_t>(workers)) workers = static_cast<int>(most_tiles);
+  return col::launch_serialised(kernel, dim3(static_cast<unsigned>(workers * CG)),
+                                dim3(col::sm100::kCtaThreads), Cfg::kSmemBytes, s, p);
+}
+
+// Tensor-core product; -1 where TMA cannot address the operands.
+template <bool SWIGLU>
+int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
+           const std::int32_t* offsets, void* out, std::uint64_t t, std::uint64_t k,
+           std::uint64_t n, std::uint64_t experts, cudaStream_t s) {
+  const std::uint64_t w_rows = SWIGLU ? 2 * n : n;
+  if (!tma_ok(x, k, 1) || !tma_ok(w, k, 1)) return -1;
+  int dev = 0;
+  const col::DeviceInfo& info = col::device_info(&dev);
+  if (info.cc_major != 10) return col::kErrDeviceNotSupported;
+  col::sm100::Fp8Params fp;
+  std::memset(&fp, 0, sizeof(fp));
+  GroupedParams& p = fp.g;
+  p.status = col::gemm_status_ptr(dev);
+  if (!p.status) return static_cast<int>(cudaErrorInvalidDevice);
+  p.offsets = offsets;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.rows = static_cast<int>(t);
+  p.groups = static_cast<int>(experts);
+  p.out_cols = static_cast<int>(n);
+  p.num_k_blocks = static_cast<int>((k + 127) / 128);
+  p.up_offset = static_cast<int>(n);
+  p.out_vec_ok = col::aligned16(out) && n % 8 == 0;
+  fp.a_scale = xs;
+  fp.b_scale = ws;
+  fp.b_scale_rows = static_cast<int>((w_rows + 127) / 128);
+
+  int cg = t >= 256 * experts ? 2 : 1;
+  int bn = cg == 2 ? 256 : 128;
+  if (const char* force = std::getenv("GROUPED_VARIANT")) {
+    cg = force[0] - '0';
+    bn = std::atoi(force + 1);
+  }
+  p.num_n_blocks = static_cast<int>((w_rows + bn - 1) / bn);
+  const std::uint64_t most_tiles = (t / (128 * cg) + experts) * p.num_n_blocks;
+  if (most_tiles > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
+  int rc = encode_map(&p.map_a, {x, k, t, 0, cg == 1 ? 32u : 128u, 1});
+  if (rc == 0) rc = encode_map(&p.map_b, {w, k, w_rows, experts, static_cast<std::uint32_t>(bn / 2), 1});
+  if (rc != 0) return rc;
+  if (cg == 2) {
+    if (bn == 256) return launch_fp8<SWIGLU, 2, 256>(fp, most_tiles, dev, info.sm_count, s);
+    return launch_fp8<SWIGLU, 2, 128>(fp, most_tiles, dev, info.sm_count, s);
+  }
+  if (bn == 256) return launch_fp8<SWIGLU, 1, 256>(fp, most_tiles, dev, info.sm_count, s);
+  return launch_fp8<SWIGLU, 1, 128>(fp, most_tiles, dev, info.sm_count, s);
+}
+
 template <bool SWIGLU>
 int grouped_forward_bf16(const void* x, const void* w, const std::int32_t* offsets, void* out,
                          std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
@@ -235,11 +310,13 @@ int forward_fp8(const void* x, const float* xs, const void* w, const float* ws,
   }
   // A tile of scales must not span gate and up rows.
   if (SWIGLU && n % 128 != 0) return static_cast<int>(cudaErrorInvalidValue);
+  const cudaStream_t s = col::as_stream(stream);
+  const int rc = fp8_tc<SWIGLU>(x, xs, w, ws, offsets, out, t, k, n, experts, s);
+  if (rc != -1) return rc;
   GroupedSimtParams p = simt_params(x, w, offsets, out, t, k, n, w_rows, experts);
   p.a_scale = xs;
   p.b_scale = ws;
-  return col::simt::launch_grouped_simt<__nv_fp8_e4m3, col::simt::kForward, SWIGLU>(
-      p, col::as_stream(stream));
+  return col::simt::launch_grouped_simt<__nv_fp8_e4m3, col::simt::kForward, SWIGLU>(p, s);
 }
 
 }  // namespace
