@@ -115,6 +115,8 @@ int allow_smem(Kernel kernel, std::uint32_t bytes, int dev, std::atomic<std::uin
 }
 
 // Workers (CTAs or CTA pairs) that can be resident at once.
+// (every kernel here takes over half of an SM's shared memory, so one answer a
+// device serves them all)
 template <typename Kernel>
 int resident_pairs(Kernel kernel, std::uint32_t smem, int dev) {
   static std::atomic<int> cached[64] = {};
@@ -223,7 +225,7 @@ int launch_fp8(col::sm100::Fp8Params& p, std::uint64_t most_tiles, int dev, int 
     static const bool covered = [kernel]() {
       cudaFuncAttributes attr;
       return cudaFuncGetAttributes(&attr, kernel) == cudaSuccess &&
-             attr.numRegs >= col::sm100::kRegsLaunchNeeded;
+             attr.numRegs >= col::sm100::kFp8RegsLaunch;
     }();
     if (!covered) return static_cast<int>(cudaErrorInvalidConfiguration);
   }
@@ -273,7 +275,8 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
   p.num_n_blocks = static_cast<int>((w_rows + bn - 1) / bn);
   const std::uint64_t most_tiles = (t / (128 * cg) + experts) * p.num_n_blocks;
   if (most_tiles > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
-  int rc = encode_map(&p.map_a, {x, k, t, 0, cg == 1 ? 32u : 128u, 1});
+  int rc = encode_map(&p.map_a, {x, k, t, 0, 128, 1});
+  if (rc == 0) rc = encode_map(&fp.map_a32, {x, k, t, 0, 32, 1});
   if (rc == 0) rc = encode_map(&p.map_b, {w, k, w_rows, experts, static_cast<std::uint32_t>(bn / 2), 1});
   if (rc != 0) return rc;
   if (cg == 2) {

@@ -124,6 +124,54 @@ __device__ __forceinline__ void grouped_commit(uint32_t bar) {
   }
 }
 
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
+// Bounded wait of a whole converged warp (mbar_wait is one thread's).  All
+// lanes poll with one instruction, read one flag and count alike, so that they
+// leave together; a count needs no registers for clocks, of which the e4m3
+// kernel's readers have none to spare.  2^24 polls are a quarter of a second
+// at the least.
+constexpr uint32_t kWarpWaitPolls = 1u << 24;
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 0u && *abort_flag) break;
+  }
+  return false;
+}
+
+// Arrival on a barrier of the cluster that publishes no memory.
+__device__ __forceinline__ void arrive_relaxed_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+// This warp has read its part of a partial sum: one arrival for the MMA issuer
+// (of CTA 0).  Only tensor-memory reads come before it, which the fence orders,
+// so the arrival itself is relaxed: with release semantics at cluster scope a
+// block took 0.8 us where this takes 0.5 (8192 x 4096 x 4096, CTA pairs).
+template <int CG>
+__device__ __forceinline__ void release_sum(uint32_t bar, int lane) {
+  tc_fence_before();
+  __syncwarp();
+  if (lane == 0) {
+    if constexpr (CG == 2) {
+      arrive_relaxed_cluster(bar);
+    } else {
+      mbar_arrive(bar);
+    }
+  }
+}
+
 // What the roles share about one tile.
 struct GroupedTile {
   int group;
@@ -168,23 +216,75 @@ __device__ __forceinline__ int ragged_rows(const GroupedTile& t) {
   return last % 16 == 0 ? 0 : last;
 }
 
-// One row of W consecutive outputs.
-template <int W>
-__device__ __forceinline__ void grouped_store(const GroupedParams& p, std::size_t row, int col0,
-                                              const float (&o)[W]) {
-  __nv_bfloat16* dst = p.out + row * p.out_cols + col0;
-  if (p.out_vec_ok && col0 + W <= p.out_cols) {
-    uint4* d4 = reinterpret_cast<uint4*>(dst);
+// ---------------------------------------------------------------- output
+//
+// A lane of an epilogue warp holds one output row, so storing straight from
+// its registers would write 32 rows 16 bytes at a time: half sectors, 32 lines
+// an instruction (an 8192 x 4096 x 4096 e4m3 product spent 36 of 167 us on
+// it).  The lanes exchange words first, so that neighbouring lanes hold
+// neighbouring columns of a row.
+
+// Within each N lanes: unit i (UNIT words) of lane l to unit l of lane i.
+template <int N, int UNIT>
+__device__ __forceinline__ void lane_transpose(uint32_t (&w)[N * UNIT], int lane) {
 #pragma unroll
-    for (int j = 0; j < W / 8; ++j) {
-      d4[j] = make_uint4(pack_bf16x2(o[8 * j], o[8 * j + 1]), pack_bf16x2(o[8 * j + 2], o[8 * j + 3]),
-                         pack_bf16x2(o[8 * j + 4], o[8 * j + 5]),
-                         pack_bf16x2(o[8 * j + 6], o[8 * j + 7]));
+  for (int bit = 1; bit < N; bit <<= 1) {
+    const bool upper = (lane & bit) != 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (i & bit) continue;
+#pragma unroll
+      for (int u = 0; u < UNIT; ++u) {
+        uint32_t& lo = w[i * UNIT + u];
+        uint32_t& hi = w[(i | bit) * UNIT + u];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? lo : hi, bit);
+        if (upper) {
+          lo = got;
+        } else {
+          hi = got;
+        }
+      }
+    }
+  }
+}
+
+// 64 output columns (32 words of two) of the warp's 32 rows, from column col0:
+// lane l holds row l; rows from `valid` on and columns from p.out_cols on are
+// not stored.  All lanes call it.
+__device__ __forceinline__ void store_rows64(const GroupedParams& p, std::size_t row0, int valid,
+                                             int col0, int cols, uint32_t (&w)[32], int lane) {
+  __nv_bfloat16* base = p.out + row0 * p.out_cols + col0;
+  const int limit = min(cols, p.out_cols - col0);  // columns to store
+  if (p.out_vec_ok) {
+    // four lanes' 16-byte pieces of a row side by side: 64-byte runs
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      uint32_t v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = w[16 * g + i];
+      lane_transpose<4, 4>(v, lane);
+      const int c = 32 * g + 8 * (lane & 3);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = (lane & ~3) + j;
+        if (r < valid && c < limit) {
+          *reinterpret_cast<uint4*>(base + static_cast<std::size_t>(r) * p.out_cols + c) =
+              make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+      }
     }
   } else {
+    // rows of any alignment: a row's 64 columns over the 32 lanes
+    lane_transpose<32, 1>(w, lane);
+    const int c = 2 * lane;
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      if (col0 + j < p.out_cols) dst[j] = __float2bfloat16_rn(o[j]);
+    for (int r = 0; r < 32; ++r) {
+      if (r < valid) {
+        __nv_bfloat16* dst = base + static_cast<std::size_t>(r) * p.out_cols + c;
+        const uint32_t v = w[r];
+        if (c < limit) *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(v);
+        if (c + 1 < limit) *reinterpret_cast<uint16_t*>(dst + 1) = static_cast<uint16_t>(v >> 16);
+      }
     }
   }
 }
@@ -313,7 +413,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
           } else if (leader) {
             mbar_arrive_expect_tx(fb_local, CG * bytes);
           } else if constexpr (MODE == kGradW) {
-            mbar_arrive_cluster(fb);
+            arrive_relaxed_cluster(fb);  // it orders nothing: the bytes are counted by CTA 0
           }
 #pragma unroll
           for (int j = 0; j < kKps; ++j) {
@@ -377,8 +477,9 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
-      // ---------------- MMA issuer
+    if (leader) {
+      // ---------------- MMA issuer: the whole warp keeps the loop's state, so that
+      // the descriptors stay in uniform registers; one lane issues
       int stage = 0;
       uint32_t phase = 0;
       int local = 0;
@@ -388,8 +489,8 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
         const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
         if (MODE == kGradW && t.k_blocks == 0) continue;  // zeros, stored without a sum
         const int acc = local & 1;
-        if (!mbar_wait(smem_u32(tempty_bar + acc), ((local >> 1) & 1) ^ 1u, abort_flag)) {
-          fail(kStatusMma);
+        if (!warp_wait(smem_u32(tempty_bar + acc), ((local >> 1) & 1) ^ 1u, abort_flag)) {
+          if (lane == 0) fail(kStatusMma);
           break;
         }
         ++local;
@@ -397,46 +498,50 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
         const uint32_t d_tmem = tmem_base + acc * BN;
         const int last_rows = MODE == kGradW ? t.end - t.begin - (t.k_blocks - 1) * kBlockK : 0;
         for (int kb = 0; kb < t.k_blocks; kb += kKps) {
-          if (!mbar_wait(smem_u32(full_bar + stage), phase, abort_flag)) {
-            fail(kStatusMma);
+          if (!warp_wait(smem_u32(full_bar + stage), phase, abort_flag)) {
+            if (lane == 0) fail(kStatusMma);
             ok = false;
             break;
           }
           tc_fence_after();
           const int nk = min(kKps, t.k_blocks - kb);
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kKps; ++j) {
-            if (j >= nk) break;
-            const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
-            const uint32_t sb = sa + Cfg::kABytes;
-            int steps = kBlockK / 16;
-            if (MODE == kGradW && kb + j == t.k_blocks - 1) steps = (last_rows + 15) / 16;
+            for (int j = 0; j < kKps; ++j) {
+              if (j >= nk) break;
+              const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
+              const uint32_t sb = sa + Cfg::kABytes;
+              int steps = kBlockK / 16;
+              if (MODE == kGradW && kb + j == t.k_blocks - 1) steps = (last_rows + 15) / 16;
 #pragma unroll
-            for (int k = 0; k < kBlockK / 16; ++k) {
-              if (MODE == kGradW && k >= steps) break;
-              const uint64_t ad = MODE == kGradW ? sdesc_mnmajor_sw128(sa + k * 2048, kChunkBytes)
-                                                 : sdesc_kmajor_sw128(sa + k * 32);
-              const uint64_t bd = MODE == kForward ? sdesc_kmajor_sw128(sb + k * 32)
-                                                   : sdesc_mnmajor_sw128(sb + k * 2048, kChunkBytes);
-              const uint32_t accumulate = (kb + j != 0 || k != 0) ? 1u : 0u;
-              if constexpr (CG == 2) {
-                umma_bf16_pair(d_tmem, ad, bd, kIdesc, accumulate);
-              } else {
-                umma_bf16(d_tmem, ad, bd, kIdesc, accumulate);
+              for (int k = 0; k < kBlockK / 16; ++k) {
+                if (MODE == kGradW && k >= steps) break;
+                const uint64_t ad = MODE == kGradW ? sdesc_mnmajor_sw128(sa + k * 2048, kChunkBytes)
+                                                   : sdesc_kmajor_sw128(sa + k * 32);
+                const uint64_t bd = MODE == kForward ? sdesc_kmajor_sw128(sb + k * 32)
+                                                     : sdesc_mnmajor_sw128(sb + k * 2048, kChunkBytes);
+                const uint32_t accumulate = (kb + j != 0 || k != 0) ? 1u : 0u;
+                if constexpr (CG == 2) {
+                  umma_bf16_pair(d_tmem, ad, bd, kIdesc, accumulate);
+                } else {
+                  umma_bf16(d_tmem, ad, bd, kIdesc, accumulate);
+                }
               }
             }
+            grouped_commit<CG>(smem_u32(empty_bar + stage));
           }
+          __syncwarp();
           issued_any = true;
-          grouped_commit<CG>(smem_u32(empty_bar + stage));
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
         if (!ok) break;
-        grouped_commit<CG>(smem_u32(tfull_bar + acc));
+        if (elect_one()) grouped_commit<CG>(smem_u32(tfull_bar + acc));
+        __syncwarp();
       }
-      if (issued_any) {
+      if (issued_any && elect_one()) {
         if constexpr (CG == 2) {
           umma_commit_pair_local(smem_u32(drain_bar));
         } else {
@@ -457,7 +562,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
         if (first != 0) {
           const int slot = (stage + stages - 1) % kStages;
           const bool got =
-              mbar_wait(smem_u32(tail_bar + slot), (tail_phase >> slot) & 1u, abort_flag);
+              warp_wait(smem_u32(tail_bar + slot), (tail_phase >> slot) & 1u, abort_flag);
           tail_phase ^= 1u << slot;
           if (!got) {
             if (lane == 0) fail(kStatusProducer);
@@ -495,14 +600,22 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     int local = 0;
     for (int tile = worker; tile < num_tiles; tile += workers) {
       const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
-      const int row = t.a_row + q * 32 + lane;
-      const bool row_ok = row < (MODE == kGradW ? p.out_rows : t.end);
+      const int row0 = t.a_row + q * 32;
+      // rows of this warp to store; none: they all lie behind the group's last
+      const int valid = min((MODE == kGradW ? p.out_rows : t.end) - row0, 32);
       const std::size_t out_row =
-          MODE == kGradW ? static_cast<std::size_t>(t.group) * p.out_rows + row : row;
+          MODE == kGradW ? static_cast<std::size_t>(t.group) * p.out_rows + row0 : row0;
+      // output columns of the tile and of this warp
+      constexpr int kOut = SWIGLU ? BN / 2 : BN;
+      constexpr int kMine = kOut / 2;
+      constexpr int kRun = kMine < 64 ? kMine : 64;
+      const int mine = half * kMine;
       if (MODE == kGradW && t.k_blocks == 0) {
-        const float zero[16] = {};
-        for (int c = half * 16; c < BN; c += 32) {
-          if (row_ok) grouped_store<16>(p, out_row, t.col + c, zero);
+        uint32_t w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = 0u;
+        for (int c = mine; c < mine + kMine; c += kRun) {
+          store_rows64(p, out_row, valid, t.col + c, kRun, w, lane);
         }
         continue;
       }
@@ -514,39 +627,40 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       ++local;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
-      // a warp whose rows all lie behind the group's last has nothing to store
-      if (__any_sync(0xffffffffu, row_ok)) {
-        if constexpr (SWIGLU) {
+      if (valid > 0) {
 #pragma unroll 1
-          for (int c = half * 16; c < BN / 2; c += 32) {
-            uint32_t g[16], u[16];
-            tmem_ld16x2(t_row + c, t_row + BN / 2 + c, g, u);
-            float o[16];
+        for (int c = mine; c < mine + kMine; c += kRun) {
+          uint32_t w[32];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = silu_fast(__uint_as_float(g[j])) * __uint_as_float(u[j]);
-            if (row_ok) grouped_store<16>(p, out_row, t.col + c, o);
-          }
-        } else {
-#pragma unroll 1
-          for (int c = half * 32; c < BN; c += 64) {
-            uint32_t a[32];
-            tmem_ld32(t_row + c, a);
-            float o[32];
+          for (int i = 0; i < 32; ++i) w[i] = 0u;
+          if constexpr (SWIGLU) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __uint_as_float(a[j]);
-            if (row_ok) grouped_store<32>(p, out_row, t.col + c, o);
+            for (int h = 0; h < kRun; h += 16) {
+              uint32_t g[16], u[16];
+              tmem_ld16x2(t_row + c + h, t_row + BN / 2 + c + h, g, u);
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                w[(h + j) / 2] = pack_bf16x2(
+                    silu_fast(__uint_as_float(g[j])) * __uint_as_float(u[j]),
+                    silu_fast(__uint_as_float(g[j + 1])) * __uint_as_float(u[j + 1]));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int h = 0; h < kRun; h += 32) {
+              uint32_t a[32];
+              tmem_ld32(t_row + c + h, a);
+#pragma unroll
+              for (int j = 0; j < 32; j += 2) {
+                w[(h + j) / 2] = pack_bf16x2(__uint_as_float(a[j]), __uint_as_float(a[j + 1]));
+              }
+            }
           }
+          store_rows64(p, out_row, valid, t.col + c, kRun, w, lane);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if constexpr (CG == 2) {
-          mbar_arrive_cluster(map_to_cta(smem_u32(tempty_bar + acc), 0));
-        } else {
-          mbar_arrive(smem_u32(tempty_bar + acc));
-        }
-      }
+      const uint32_t bar = smem_u32(tempty_bar + acc);
+      release_sum<CG>(CG == 2 ? map_to_cta(bar, 0) : bar, lane);
     }
   }
 
