@@ -17,13 +17,13 @@
 #pragma once
 
 #include "gemm_grouped_sm100.cuh"
+#include "gemm_sm100_sk.cuh"
 
 namespace col {
 namespace sm100 {
 
 struct __align__(64) Fp8Params {
-  GroupedParams g;       // map_a: boxes of 128 rows
-  CUtensorMap map_a32;   // the same in boxes of 32 rows
+  GroupedParams g;
   const float* a_scale;  // [rows, k_blocks]
   const float* b_scale;  // [groups, b_scale_rows, k_blocks]
   int b_scale_rows;
@@ -40,23 +40,38 @@ constexpr int kFp8RegsReader = 232;
 constexpr int kFp8RegsLaunch = 168;
 static_assert(128 * kFp8RegsControl + 256 * kFp8RegsReader <= 384 * kFp8RegsLaunch, "register shares");
 
-template <int CG, int BN>
+// ROWS = 32: tiles of at most 32 rows, for products whose time is reading w.
+// Only those rows of A are loaded and kept (the MMA's other 96 rows read
+// whatever lies behind them; what they add up is not stored), which leaves the
+// ring to w.  SPLIT: the CTAs of a cluster share a tile's k-blocks and add
+// their sums up in the first one, for a few such tiles.
+template <int CG, int BN, int ROWS, int SPLIT>
 struct Fp8Cfg {
-  static constexpr int kTileRows = kBlockM * CG;
-  static constexpr uint32_t kABytes = kBlockM * kFp8BlockK;
+  static_assert((ROWS == kBlockM && SPLIT == 1) || (ROWS == 32 && CG == 1), "variants");
+  static constexpr int kTileRows = ROWS * CG;
+  static constexpr int kCols = BN / 2;  // accumulator columns of a reading thread
+  static constexpr int kChunk = kCols < 64 ? kCols / 2 : 32;  // columns read at a time
+  static constexpr uint32_t kABytes = ROWS * kFp8BlockK;
   static constexpr uint32_t kBBytes = BN / CG * kFp8BlockK;
   static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
-  static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : 2;  // k-blocks a stage
+  // k-blocks a stage
+  static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : (BN == 64 ? 4 : 2);
   static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
-  static constexpr uint32_t kExtraBytes = 512 + kGroupedTableBytes;
+  // one warp's sums of 32 rows, from each other CTA, for two warps
+  static constexpr uint32_t kSumBytes = 32 * kCols * 4;
+  static constexpr uint32_t kExtraBytes = 512 + kGroupedTableBytes + (SPLIT - 1) * 2 * kSumBytes;
   static constexpr int kStagesFit =
       static_cast<int>((kSmemLimit - 1024 - kExtraBytes) / kStageBytes);
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
-  static constexpr int kAccs = 512 / BN;  // partial sums in flight
+  // Partial sums are handed over in groups: a whole stage's where TMEM holds two
+  // such groups, else one by one.  A hand-over costs the issuing warp ~300
+  // cycles (two waits, a commit) beside ~35 for each MMA.
+  static constexpr int kGroup = 512 / BN / kKps >= 2 ? kKps : 1;
+  static constexpr int kAccs = 512 / BN / kGroup;  // groups in flight
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024 + kExtraBytes;
-  static constexpr int kSlots = kStages * kKps;  // k-blocks in the ring
+  static constexpr int kSlots = kStages * kKps / kGroup;  // groups in the ring
   static_assert(kSlots >= kAccs && kSlots <= 32, "a slot outlives its partial sum");
-  static_assert((kStages + kSlots + kAccs + 1) * 8 + 8 <= 512, "barrier space");
+  static_assert((kStages + kSlots + kAccs + 3) * 8 + 8 <= 512 && kKps / kGroup <= 2, "barrier space");
 };
 
 // Instruction descriptor, kind::f8f6f4: D fp32, A and B e4m3, both K-major.
@@ -84,8 +99,12 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t adesc, uint6
   }
 }
 
-// tcgen05.ld of 32 columns without waiting; tmem_ld_wait completes it and names
-// the registers, so that no use of them is scheduled before it.
+// tcgen05.ld of 16 or 32 columns without waiting; tmem_ld_wait completes it and
+// names the registers, so that no use of them is scheduled before it.
+__device__ __forceinline__ void tmem_ld_start(uint32_t taddr, uint32_t (&r)[16]) {
+  tmem_ld16_start(taddr, r);
+}
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[16]) { tmem_wait16(r); }
 __device__ __forceinline__ void tmem_ld_start(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -112,6 +131,22 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                : "memory");
 }
 
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+
+// warp_wait on data that other CTAs of the cluster wrote.
+__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity,
+                                                  volatile int* abort_flag) {
+  for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if ((i & 63u) == 0u && *abort_flag) break;
+  }
+  return false;
+}
+
 // sums += part * scale, two columns an instruction.
 template <int W>
 __device__ __forceinline__ void add_scaled(uint64_t* sums, const uint32_t (&part)[W], float scale) {
@@ -131,17 +166,19 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
   return f;
 }
 
-constexpr int kChunk = 32;  // columns of a partial sum read at a time
 
-template <bool SWIGLU, int CG, int BN>
-__global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
+template <bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
+__global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads, 1)
     fp8_kernel(const __grid_constant__ Fp8Params fp) {
-  using Cfg = Fp8Cfg<CG, BN>;
+  using Cfg = Fp8Cfg<CG, BN, ROWS, SPLIT>;
   const GroupedParams& p = fp.g;
   constexpr int kStages = Cfg::kStages;
   constexpr int kKps = Cfg::kKps;
   constexpr int kAccs = Cfg::kAccs;
-  constexpr uint32_t kIdesc = idesc_e4m3_f32(Cfg::kTileRows, BN);
+  constexpr int kGroup = Cfg::kGroup;
+  constexpr int kGroups = kKps / kGroup;  // a stage
+  constexpr bool kWrap = ROWS == 32 && SPLIT == 1;  // sums start at first_k
+  constexpr uint32_t kIdesc = idesc_e4m3_f32(kBlockM * CG, BN);
   constexpr bool kSplitRegs = fp8_split_regs(BN);
 
   extern __shared__ uint8_t smem_raw[];
@@ -149,30 +186,38 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       (reinterpret_cast<std::uintptr_t>(smem_raw) + 1023) & ~static_cast<std::uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * Cfg::kStageBytes);
   uint64_t* full_bar = bars;
-  // One barrier a k-block in the ring says that its MMAs are done: the warps
-  // that read the partial sum wait for it, and the producer before it refills
-  // the slot.  (A second commit for the producer cost ~0.1 us a block.)  No
-  // waiter can miss a phase: a slot is used again only after its partial sum
-  // was read, as there are at least as many slots as accumulators.
+  // One barrier a group in the ring says that its MMAs are done: the warps that
+  // read the partial sums wait for it, and the producer before it refills the
+  // stage.  (A second commit for the producer cost ~0.1 us a block.)  No waiter
+  // can miss a phase: a slot is used again only after its partial sums were
+  // read, as there are at least as many slots as groups of accumulators.
   uint64_t* done_bar = bars + kStages;
   uint64_t* tempty_bar = done_bar + Cfg::kSlots;
   uint64_t* drain_bar = tempty_bar + kAccs;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  uint64_t* sums_bar = drain_bar + 1;  // the other CTAs' sums for each of two warps
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sums_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   int* prefix = reinterpret_cast<int*>(smem + kStages * Cfg::kStageBytes + 512);
+  uint8_t* other_sums = smem + kStages * Cfg::kStageBytes + 512 + kGroupedTableBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
   const bool leader = rank == 0;
-  const int worker = blockIdx.x / CG;
-  const int workers = gridDim.x / CG;
+  const int worker = blockIdx.x / (CG * SPLIT);
+  const int workers = gridDim.x / (CG * SPLIT);  // SPLIT > 1: at least as many as tiles
+  // this CTA's k-blocks
+  const int share = SPLIT > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int kb_begin = p.num_k_blocks * share / SPLIT;
+  const int kb_end = p.num_k_blocks * (share + 1) / SPLIT;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(full_bar + s), 1);
     for (int s = 0; s < Cfg::kSlots; ++s) mbar_init(smem_u32(done_bar + s), 1);
     for (int a = 0; a < kAccs; ++a) mbar_init(smem_u32(tempty_bar + a), CG * kEpiWarps);
     mbar_init(smem_u32(drain_bar), 1);
+    mbar_init(smem_u32(sums_bar), 1);
+    mbar_init(smem_u32(sums_bar + 1), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     grid_dependents_launch();
@@ -189,7 +234,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     fill_tile_prefix(prefix, p.offsets, p.groups, p.rows, Cfg::kTileRows, lane);
   }
   tc_fence_before();
-  if constexpr (CG == 2) {
+  if constexpr (CG * SPLIT > 1) {
     cluster_sync();
   } else {
     __syncthreads();
@@ -205,36 +250,39 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   if (warp < 4) {
     if constexpr (kSplitRegs) regs_release<kFp8RegsControl>();
     if (warp == 0) {
-      if (lane == 0) {
-        // ---------------- TMA producer
+      // ---------------- TMA producer: the whole warp keeps the loop's state, so
+      // that addresses and coordinates stay in uniform registers; one lane issues
+      if (elect_one()) {
         prefetch_tmap(&p.map_a);
         prefetch_tmap(&p.map_b);
-        int stage = 0;
-        uint32_t phase = 0;
-        uint32_t issued_mask = 0;
-        uint32_t issued_phase = 0;
-        uint32_t slot_phase = 0;  // bit s: parity of slot s's next use
-        uint32_t last_slots = 0;  // two bits a stage: its last k-block in use
-        int filled = 0;
-        bool ok = true;
-        for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-          const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN>(p, prefix, tile, rank);
-          // Single CTAs load A 32 rows at a time where the group ends early.
-          const int rows = min(kBlockM, (t.end - t.a_row + 31) & ~31);
-          const bool whole = CG == 2 || rows == kBlockM;
-          for (int kb = 0; kb < t.k_blocks; kb += kKps) {
-            const int nk = min(kKps, t.k_blocks - kb);
-            if (filled >= kStages) {
-              const int last = last_slots >> (2 * stage) & 3;
-              const int slot = stage * kKps + last;
-              if (!mbar_wait(smem_u32(done_bar + slot), ((slot_phase >> slot) & 1u) ^ 1u, abort_flag)) {
-                fail(kStatusProducer);
-                ok = false;
-                break;
-              }
-            } else {
-              ++filled;
+      }
+      __syncwarp();
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t issued_mask = 0;
+      uint32_t issued_phase = 0;
+      uint32_t slot_phase = 0;  // bit s: parity of slot s's next use
+      uint32_t last_slots = 0;  // two bits a stage: its last group in use
+      int filled = 0;
+      bool ok = true;
+      for (int tile = worker; ok && tile < num_tiles; tile += workers) {
+        const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+        // Single CTAs load A 32 rows at a time where the group ends early.
+        const int rows = min(ROWS, (t.end - t.a_row + 31) & ~31);
+        const bool whole = CG == 2 || rows == kBlockM;
+        for (int kb = kb_begin; kb < kb_end; kb += kKps) {
+          const int nk = min(kKps, kb_end - kb);
+          if (filled >= kStages) {
+            const int slot = stage * kGroups + static_cast<int>(last_slots >> (2 * stage) & 3u);
+            if (!warp_wait(smem_u32(done_bar + slot), ((slot_phase >> slot) & 1u) ^ 1u, abort_flag)) {
+              if (lane == 0) fail(kStatusProducer);
+              ok = false;
+              break;
             }
+          } else {
+            ++filled;
+          }
+          if (elect_one()) {
             const uint32_t bytes = nk * ((whole ? kBlockM : rows) * 128u + Cfg::kBBytes);
             const uint32_t fb_local = smem_u32(full_bar + stage);
             uint32_t fb = fb_local;
@@ -245,43 +293,54 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
               if (j >= nk) break;
               const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
               const uint32_t sb = sa + Cfg::kABytes;
-              const int kc = (kb + j) * kFp8BlockK;
+              int kc = kb + j;
+              if constexpr (kWrap) {
+                kc += t.first_k;
+                if (kc >= kb_end) kc -= kb_end;
+              }
+              kc *= kFp8BlockK;
               if (whole) {
                 grouped_load_2d<CG>(sa, &p.map_a, fb, kc, t.a_row);
               } else {
                 for (int r = 0; r < rows; r += 32) {
-                  grouped_load_2d<CG>(sa + r * 128, &fp.map_a32, fb, kc, t.a_row + r);
+                  grouped_load_2d<CG>(sa + r * 128, &p.map_a32, fb, kc, t.a_row + r);
                 }
               }
+              constexpr int kBoxRows = b_box_rows(SWIGLU, CG, BN);
 #pragma unroll
-              for (int i = 0; i < 2 / CG; ++i) {
+              for (int i = 0; i < BN / CG / kBoxRows; ++i) {
                 const int h = CG == 2 ? rank : i;
-                grouped_load_3d<CG>(sb + i * (BN / 2 * 128), &p.map_b, fb, kc,
+                grouped_load_3d<CG>(sb + i * (kBoxRows * 128), &p.map_b, fb, kc,
                                     t.col + h * (SWIGLU ? p.up_offset : BN / 2), t.group);
               }
-              slot_phase ^= 1u << (stage * kKps + j);
             }
-            last_slots = (last_slots & ~(3u << (2 * stage))) | (static_cast<uint32_t>(nk - 1) << (2 * stage));
-            issued_mask |= 1u << stage;
-            issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-            if (++stage == kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
+          }
+          __syncwarp();
+          const int last = (nk - 1) / kGroup;
+#pragma unroll
+          for (int i = 0; i < kGroups; ++i) {
+            if (i <= last) slot_phase ^= 1u << (stage * kGroups + i);
+          }
+          last_slots = (last_slots & ~(3u << (2 * stage))) | (static_cast<uint32_t>(last) << (2 * stage));
+          issued_mask |= 1u << stage;
+          issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
           }
         }
-        if (!ok || *abort_flag) {
-          if (leader) {
-            for (int s = 0; s < kStages; ++s) {
-              if ((issued_mask & (1u << s)) &&
-                  !mbar_wait_drain(smem_u32(full_bar + s), (issued_phase >> s) & 1u)) {
-                atomicOr(p.status, kStatusDrain);
-              }
+      }
+      if (lane == 0 && (!ok || *abort_flag)) {
+        if (leader) {
+          for (int s = 0; s < kStages; ++s) {
+            if ((issued_mask & (1u << s)) &&
+                !mbar_wait_drain(smem_u32(full_bar + s), (issued_phase >> s) & 1u)) {
+              atomicOr(p.status, kStatusDrain);
             }
-          } else {
-            // CTA 1 cannot observe CTA 0's barriers: give its copies time to land.
-            for (int i = 0; i < 200; ++i) __nanosleep(1000);
           }
+        } else {
+          // CTA 1 cannot observe CTA 0's barriers: give its copies time to land.
+          for (int i = 0; i < 200; ++i) __nanosleep(1000);
         }
       }
     } else if (warp == 1) {
@@ -295,31 +354,36 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
         bool ok = true;
         bool issued_any = false;
         for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-          for (int kb = 0; ok && kb < p.num_k_blocks; kb += kKps) {
+          for (int kb = kb_begin; ok && kb < kb_end; kb += kKps) {
             if (!warp_wait(smem_u32(full_bar + stage), phase, abort_flag)) {
               if (lane == 0) fail(kStatusMma);
               ok = false;
               break;
             }
 #pragma unroll
-            for (int j = 0; j < kKps; ++j) {
-              if (kb + j >= p.num_k_blocks) break;
+            for (int g = 0; g < kGroups; ++g) {
+              if (kb + g * kGroup >= kb_end) break;
               if (!warp_wait(smem_u32(tempty_bar + acc), acc_phase ^ 1u, abort_flag)) {
                 if (lane == 0) fail(kStatusMma);
                 ok = false;
                 break;
               }
               tc_fence_after();
-              const uint32_t d_tmem = tmem_base + acc * BN;
-              const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
-              const uint32_t sb = sa + Cfg::kABytes;
               if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kFp8BlockK / 32; ++k) {
-                  umma_e4m3<CG>(d_tmem, sdesc_kmajor_sw128(sa + k * 32),
-                                sdesc_kmajor_sw128(sb + k * 32), kIdesc, k != 0 ? 1u : 0u);
+                for (int i = 0; i < kGroup; ++i) {
+                  const int j = g * kGroup + i;
+                  if (i > 0 && kb + j >= kb_end) break;
+                  const uint32_t d_tmem = tmem_base + (acc * kGroup + i) * BN;
+                  const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
+                  const uint32_t sb = sa + Cfg::kABytes;
+#pragma unroll
+                  for (int k = 0; k < kFp8BlockK / 32; ++k) {
+                    umma_e4m3<CG>(d_tmem, sdesc_kmajor_sw128(sa + k * 32),
+                                  sdesc_kmajor_sw128(sb + k * 32), kIdesc, k != 0 ? 1u : 0u);
+                  }
                 }
-                grouped_commit<CG>(smem_u32(done_bar + stage * kKps + j));
+                grouped_commit<CG>(smem_u32(done_bar + stage * kGroups + g));
               }
               __syncwarp();
               issued_any = true;
@@ -347,7 +411,8 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   } else {
     // ---------------- sums and epilogue: this CTA's 128 rows, half the columns a warpgroup
     if constexpr (kSplitRegs) regs_acquire<kFp8RegsReader>();
-    constexpr int kCols = BN / 2;  // accumulator columns of a thread
+    constexpr int kCols = Cfg::kCols;
+    constexpr int kChunk = Cfg::kChunk;
     const int q = warp & 3;
     const int part_of = (warp - 4) >> 2;  // which half of them
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
@@ -357,27 +422,34 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     uint32_t slot_phase = 0;  // bit s: parity of slot s's next completion
     bool ok = true;
     for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-      const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN>(p, prefix, tile, rank);
+      const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
       const int row = t.a_row + q * 32 + lane;
       const bool row_ok = row < t.end;
-      const int valid = min(t.end - (t.a_row + q * 32), 32);  // rows of this warp
+      // rows of this warp
+      const int valid = ROWS == 32 && q != 0 ? 0 : min(t.end - (t.a_row + q * 32), 32);
       const bool warp_ok = valid > 0;
       // offsets of the scales of this row and of this thread's rows of w (with
       // SwiGLU the gate rows', and the up rows' a constant behind them)
-      uint32_t xs = static_cast<uint32_t>(row_ok ? row : t.begin) * static_cast<uint32_t>(kb_count);
+      uint32_t xs = static_cast<uint32_t>(row_ok ? row : t.begin) * static_cast<uint32_t>(kb_count) + kb_begin;
       const int block = SWIGLU ? t.col / 128 : min((t.col + part_of * kCols) / 128, fp.b_scale_rows - 1);
-      uint32_t ws = static_cast<uint32_t>(t.group * fp.b_scale_rows + block) * static_cast<uint32_t>(kb_count);
+      uint32_t ws = static_cast<uint32_t>(t.group * fp.b_scale_rows + block) * static_cast<uint32_t>(kb_count) + kb_begin;
+      int left = kb_count;  // k-blocks until the last one's scales
+      if constexpr (kWrap) {
+        left -= t.first_k;
+        xs += t.first_k;
+        ws += t.first_k;
+      }
       const uint32_t wu = SWIGLU ? static_cast<uint32_t>(p.up_offset / 128 * kb_count) : 0u;
       uint64_t sums[kCols / 2];  // two fp32 each
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) sums[i] = 0u;
-      // The sum of the next k-block: waits until its MMAs are done.
-      auto next_sum = [&](int kb) {
+      // The next group of partial sums: waits until its MMAs are done.
+      auto next_group = [&](int kb) {
         if (!warp_wait(smem_u32(done_bar + slot), (slot_phase >> slot) & 1u, abort_flag)) return false;
         slot_phase ^= 1u << slot;
-        // the next block's slot: the stage's other one, or the next stage's first
-        if (kKps == 1 || (slot & 1) == 1 || kb + 1 == kb_count) {
-          slot = slot / kKps * kKps + kKps;
+        // the group after it: the stage's other one, or the next stage's first
+        if (kGroups == 1 || (slot & 1) == 1 || kb + 1 == kb_end) {
+          slot = slot / kGroups * kGroups + kGroups;
           if (slot == Cfg::kSlots) slot = 0;
         } else {
           ++slot;
@@ -391,14 +463,15 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
         if (++acc == kAccs) acc = 0;
       };
       if (!warp_ok) {
-        for (int kb = 0; kb < kb_count; ++kb) {
-          ok = next_sum(kb);
+        for (int kb = kb_begin; kb < kb_end; kb += kGroup) {
+          ok = next_group(kb);
           if (!ok) break;
           release();
         }
       } else {
         constexpr int kChunks = kCols / kChunk;
         static_assert(kChunks % 2 == 0, "the chunks' registers alternate");
+        int in_group = 0;
         auto chunk_addr = [&](int c) {
           uint32_t col;
           if constexpr (SWIGLU) {
@@ -409,34 +482,47 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
           } else {
             col = part_of * kCols + c * kChunk;
           }
-          return t_lane + acc * BN + col;
+          return t_lane + (acc * kGroup + in_group) * BN + col;
         };
         float next_x = __ldg(fp.a_scale + xs);
         float next_w = __ldg(fp.b_scale + ws);
         float next_u = SWIGLU ? __ldg(fp.b_scale + ws + wu) : 0.0f;
         uint32_t part[2][kChunk];
-        ok = next_sum(0);
+        ok = next_group(kb_begin);
         if (ok) tmem_ld_start(chunk_addr(0), part[0]);
 #pragma unroll 1
-        for (int kb = 0; ok && kb < kb_count; ++kb) {
+        for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
           const float sw = next_x * next_w;
           const float su = next_x * next_u;
-          if (kb + 1 < kb_count) {
-            next_x = __ldg(fp.a_scale + ++xs);
-            next_w = __ldg(fp.b_scale + ++ws);
+          if (kb + 1 < kb_end) {
+            ++xs;
+            ++ws;
+            if constexpr (kWrap) {
+              if (--left == 0) {
+                xs -= kb_count;
+                ws -= kb_count;
+              }
+            }
+            next_x = __ldg(fp.a_scale + xs);
+            next_w = __ldg(fp.b_scale + ws);
             if constexpr (SWIGLU) next_u = __ldg(fp.b_scale + ws + wu);
           }
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             tmem_ld_wait(part[c & 1]);
             // the next load is under way while this chunk is added: the next
-            // chunk of this sum, or, once this sum is released, the next one's
+            // chunk of this sum, or the next sum's first, once this group is
+            // released where it ends
             if (c + 1 < kChunks) {
               tmem_ld_start(chunk_addr(c + 1), part[(c + 1) & 1]);
+            } else if (kGroup > 1 && in_group + 1 < kGroup && kb + 1 < kb_end) {
+              ++in_group;
+              tmem_ld_start(chunk_addr(0), part[0]);
             } else {
               release();
-              if (kb + 1 < kb_count) {
-                ok = next_sum(kb + 1);
+              in_group = 0;
+              if (kb + 1 < kb_end) {
+                ok = next_group(kb + 1);
                 if (ok) tmem_ld_start(chunk_addr(0), part[0]);
               }
             }
@@ -445,8 +531,47 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
           }
         }
       }
+      if constexpr (SPLIT > 1) {
+        // The first CTA adds the others' sums in their order.  Word j of a lane's
+        // sums from CTA s lies at ((s - 1) * 2 + part_of) * kSumBytes + (j / 4) *
+        // 512 + lane * 16: whole rows of banks for both sides.
+        if (ok && warp_ok) {
+          if (share != 0) {
+            const uint32_t to = map_to_cta(smem_u32(other_sums + ((share - 1) * 2 + part_of) * Cfg::kSumBytes), 0);
+            const uint32_t bar = map_to_cta(smem_u32(sums_bar + part_of), 0);
+            if (row_ok) {
+#pragma unroll
+              for (int j = 0; j < kCols; j += 4) {
+                st_async_v4(to + j / 4 * 512 + lane * 16, static_cast<uint32_t>(sums[j / 2]),
+                            static_cast<uint32_t>(sums[j / 2] >> 32),
+                            static_cast<uint32_t>(sums[j / 2 + 1]),
+                            static_cast<uint32_t>(sums[j / 2 + 1] >> 32), bar);
+              }
+            }
+          } else {
+            const uint32_t bar = smem_u32(sums_bar + part_of);
+            if (lane == 0) mbar_arrive_expect_tx(bar, (SPLIT - 1) * valid * kCols * 4);
+            __syncwarp();
+            ok = warp_wait_cluster(bar, 0, abort_flag);
+            if (ok && row_ok) {
+#pragma unroll 1
+              for (int from = 0; from < SPLIT - 1; ++from) {
+                const uint8_t* src = other_sums + (from * 2 + part_of) * Cfg::kSumBytes + lane * 16;
+#pragma unroll
+                for (int j = 0; j < kCols; j += 4) {
+                  const float4 v = *reinterpret_cast<const float4*>(src + j / 4 * 512);
+                  const float2 a = unpack2(sums[j / 2]);
+                  const float2 b = unpack2(sums[j / 2 + 1]);
+                  sums[j / 2] = pack2(a.x + v.x, a.y + v.y);
+                  sums[j / 2 + 1] = pack2(b.x + v.z, b.y + v.w);
+                }
+              }
+            }
+          }
+        }
+      }
       if (!ok && lane == 0) fail(kStatusEpilogue);
-      if (ok && warp_ok) {
+      if (ok && warp_ok && share == 0) {
         constexpr int kOut = SWIGLU ? kCols / 2 : kCols;
         constexpr int kRun = kOut < 64 ? kOut : 64;
 #pragma unroll
@@ -475,7 +600,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   // No CTA leaves while its partner may still address its shared memory.
   __syncwarp();
   tc_fence_before();
-  if constexpr (CG == 2) {
+  if constexpr (CG * SPLIT > 1) {
     cluster_sync();
   } else {
     __syncthreads();

@@ -1,6 +1,7 @@
 // Products grouped by expert (bf16, both gradients, block-scaled e4m3) and the
 // dense block-scaled e4m3 products, which are the same with a single group.
 #include <atomic>
+#include <cstdio>
 #include <cstdlib>
 #include <cstring>
 
@@ -141,11 +142,30 @@ int resident_pairs(Kernel kernel, std::uint32_t smem, int dev) {
   return pairs;
 }
 
-template <int MODE, bool SWIGLU, int CG, int BN>
+// A tensor-core variant: CTAs of a tile, accumulator columns, rows of a CTA,
+// CTAs that share a tile's sum.
+struct Variant {
+  int cg;
+  int bn;
+  int rows;
+  int split;
+};
+
+#ifdef EXPERIMENT
+Variant forced(Variant v) {
+  if (const char* f = std::getenv("GROUPED_VARIANT")) {
+    v.cg = f[0] - '0';
+    std::sscanf(f + 1, "%d,%d,%d", &v.bn, &v.rows, &v.split);
+  }
+  return v;
+}
+#endif
+
+template <int MODE, bool SWIGLU, int CG, int BN, int ROWS>
 int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int sm_count,
                         cudaStream_t s) {
-  using Cfg = GroupedCfg<CG, BN>;
-  auto kernel = col::sm100::grouped_bf16_kernel<MODE, SWIGLU, CG, BN>;
+  using Cfg = GroupedCfg<CG, BN, ROWS>;
+  auto kernel = col::sm100::grouped_bf16_kernel<MODE, SWIGLU, CG, BN, ROWS>;
   static std::atomic<std::uint64_t> done{0};
   if (int rc = allow_smem(kernel, Cfg::kSmemBytes, dev, done)) return rc;
   int workers = sm_count;
@@ -184,39 +204,42 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   p.up_offset = static_cast<int>(n);
   p.out_vec_ok = col::aligned16(out) && out_cols % 8 == 0;
 
-  int cg = t >= 256 * experts ? 2 : 1;
-  int bn = cg == 2 ? 256 : 128;
-  if (const char* force = std::getenv("GROUPED_VARIANT")) {
-    cg = force[0] - '0';
-    bn = std::atoi(force + 1);
-  }
-  p.num_n_blocks = static_cast<int>((out_cols * (SWIGLU ? 2 : 1) + bn - 1) / bn);
-  const std::uint64_t m_tiles = MODE == kGradW ? experts * ((n + 128 * cg - 1) / (128 * cg))
-                                               : t / (128 * cg) + experts;
+  Variant v = t >= 256 * experts ? Variant{2, 256, 128, 1} : Variant{1, 128, 128, 1};
+#ifdef EXPERIMENT
+  v = forced(v);
+#endif
+  p.num_n_blocks = static_cast<int>((out_cols * (SWIGLU ? 2 : 1) + v.bn - 1) / v.bn);
+  const std::uint64_t tile_rows = static_cast<std::uint64_t>(v.cg * v.rows);
+  const std::uint64_t m_tiles =
+      MODE == kGradW ? experts * ((n + tile_rows - 1) / tile_rows) : t / tile_rows + experts;
   const std::uint64_t most_tiles = m_tiles * p.num_n_blocks;
   if (most_tiles > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
-  const std::uint32_t a_box = MODE == kGradW ? 64 : (cg == 1 ? 32 : 128);
-  const std::uint32_t b_box = MODE == kForward ? bn / 2 : 64;
-  int rc = encode_map(&p.map_a, {a, a_cols, t, 0, a_box, 2});
+  int rc = encode_map(&p.map_a, {a, a_cols, t, 0, MODE == kGradW ? 64u : 128u, 2});
+  if (rc == 0 && MODE != kGradW && v.cg == 1) rc = encode_map(&p.map_a32, {a, a_cols, t, 0, 32, 2});
   if (rc == 0) {
+    const std::uint32_t b_box =
+        MODE == kForward ? static_cast<std::uint32_t>(col::sm100::b_box_rows(SWIGLU, v.cg, v.bn)) : 64u;
     rc = MODE == kGradW ? encode_map(&p.map_b, {b, k, t, 0, b_box, 2})
                         : encode_map(&p.map_b, {b, k, w_rows, experts, b_box, 2});
   }
   if (rc != 0) return rc;
-  if (cg == 2) {
-    if (bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 2, 256>(p, most_tiles, dev, info.sm_count, s);
-    return launch_grouped_bf16<MODE, SWIGLU, 2, 128>(p, most_tiles, dev, info.sm_count, s);
+  const int sms = info.sm_count;
+  if (v.cg == 2) return launch_grouped_bf16<MODE, SWIGLU, 2, 256, 128>(p, most_tiles, dev, sms, s);
+  if constexpr (MODE != kGradW) {
+    if (v.rows == 32) {
+      if (v.bn == 128) return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 32>(p, most_tiles, dev, sms, s);
+      return launch_grouped_bf16<MODE, SWIGLU, 1, 64, 32>(p, most_tiles, dev, sms, s);
+    }
   }
-  if (bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 1, 256>(p, most_tiles, dev, info.sm_count, s);
-  if (bn == 128) return launch_grouped_bf16<MODE, SWIGLU, 1, 128>(p, most_tiles, dev, info.sm_count, s);
-  return launch_grouped_bf16<MODE, SWIGLU, 1, 64>(p, most_tiles, dev, info.sm_count, s);
+  if (v.bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 1, 256, 128>(p, most_tiles, dev, sms, s);
+  return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 128>(p, most_tiles, dev, sms, s);
 }
 
-template <bool SWIGLU, int CG, int BN>
+template <bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
 int launch_fp8(col::sm100::Fp8Params& p, std::uint64_t most_tiles, int dev, int sm_count,
                cudaStream_t s) {
-  using Cfg = col::sm100::Fp8Cfg<CG, BN>;
-  auto kernel = col::sm100::fp8_kernel<SWIGLU, CG, BN>;
+  using Cfg = col::sm100::Fp8Cfg<CG, BN, ROWS, SPLIT>;
+  auto kernel = col::sm100::fp8_kernel<SWIGLU, CG, BN, ROWS, SPLIT>;
   static std::atomic<std::uint64_t> done{0};
   if (int rc = allow_smem(kernel, Cfg::kSmemBytes, dev, done)) return rc;
   if constexpr (col::sm100::fp8_split_regs(BN)) {
@@ -234,18 +257,25 @@ int launch_fp8(col::sm100::Fp8Params& p, std::uint64_t most_tiles, int dev, int 
     workers = resident_pairs(kernel, Cfg::kSmemBytes, dev);
     if (workers <= 0) return static_cast<int>(cudaErrorInvalidConfiguration);
   }
-  if (most_tiles < static_cast<std::uint64_t>(workers)) workers = static_cast<int>(most_tiles);
-  return col::launch_serialised(kernel, dim3(static_cast<unsigned>(workers * CG)),
+  // clusters that share a tile's sum take one tile each
+  if (SPLIT > 1 || most_tiles < static_cast<std::uint64_t>(workers)) {
+    workers = static_cast<int>(most_tiles);
+  }
+  return col::launch_serialised(kernel, dim3(static_cast<unsigned>(workers * CG * SPLIT)),
                                 dim3(col::sm100::kCtaThreads), Cfg::kSmemBytes, s, p);
 }
 
-// Tensor-core product; -1 where TMA cannot address the operands.
+// Tensor-core product; -1 where TMA cannot address the operands or 32 bits do
+// not count the scales.
 template <bool SWIGLU>
 int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
            const std::int32_t* offsets, void* out, std::uint64_t t, std::uint64_t k,
            std::uint64_t n, std::uint64_t experts, cudaStream_t s) {
   const std::uint64_t w_rows = SWIGLU ? 2 * n : n;
+  const std::uint64_t k_blocks = (k + 127) / 128;
+  const std::uint64_t scale_rows = (w_rows + 127) / 128;
   if (!tma_ok(x, k, 1) || !tma_ok(w, k, 1)) return -1;
+  if (t * k_blocks > kIntMax || experts * scale_rows * k_blocks > kIntMax) return -1;
   int dev = 0;
   const col::DeviceInfo& info = col::device_info(&dev);
   if (info.cc_major != 10) return col::kErrDeviceNotSupported;
@@ -259,32 +289,58 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
   p.rows = static_cast<int>(t);
   p.groups = static_cast<int>(experts);
   p.out_cols = static_cast<int>(n);
-  p.num_k_blocks = static_cast<int>((k + 127) / 128);
+  p.num_k_blocks = static_cast<int>(k_blocks);
   p.up_offset = static_cast<int>(n);
   p.out_vec_ok = col::aligned16(out) && n % 8 == 0;
   fp.a_scale = xs;
   fp.b_scale = ws;
-  fp.b_scale_rows = static_cast<int>((w_rows + 127) / 128);
+  fp.b_scale_rows = static_cast<int>(scale_rows);
 
-  int cg = t >= 256 * experts ? 2 : 1;
-  int bn = cg == 2 ? 256 : 128;
-  if (const char* force = std::getenv("GROUPED_VARIANT")) {
-    cg = force[0] - '0';
-    bn = std::atoi(force + 1);
-  }
-  p.num_n_blocks = static_cast<int>((w_rows + bn - 1) / bn);
-  const std::uint64_t most_tiles = (t / (128 * cg) + experts) * p.num_n_blocks;
-  if (most_tiles > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
+  Variant v = t >= 256 * experts ? Variant{2, 256, 128, 1} : Variant{1, 128, 128, 1};
+#ifdef EXPERIMENT
+  v = forced(v);
+  if (k_blocks < static_cast<std::uint64_t>(v.split)) v.split = 1;
+#endif
+  p.num_n_blocks = static_cast<int>((w_rows + v.bn - 1) / v.bn);
+  const std::uint64_t tile_rows = static_cast<std::uint64_t>(v.cg * v.rows);
+  const std::uint64_t m_tiles = offsets ? t / tile_rows + experts : (t + tile_rows - 1) / tile_rows;
+  const std::uint64_t most_tiles = m_tiles * p.num_n_blocks;
+  if (most_tiles * v.split > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
   int rc = encode_map(&p.map_a, {x, k, t, 0, 128, 1});
-  if (rc == 0) rc = encode_map(&fp.map_a32, {x, k, t, 0, 32, 1});
-  if (rc == 0) rc = encode_map(&p.map_b, {w, k, w_rows, experts, static_cast<std::uint32_t>(bn / 2), 1});
-  if (rc != 0) return rc;
-  if (cg == 2) {
-    if (bn == 256) return launch_fp8<SWIGLU, 2, 256>(fp, most_tiles, dev, info.sm_count, s);
-    return launch_fp8<SWIGLU, 2, 128>(fp, most_tiles, dev, info.sm_count, s);
+  if (rc == 0 && v.cg == 1) rc = encode_map(&p.map_a32, {x, k, t, 0, 32, 1});
+  if (rc == 0) {
+    rc = encode_map(&p.map_b, {w, k, w_rows, experts,
+                               static_cast<std::uint32_t>(col::sm100::b_box_rows(SWIGLU, v.cg, v.bn)), 1});
   }
-  if (bn == 256) return launch_fp8<SWIGLU, 1, 256>(fp, most_tiles, dev, info.sm_count, s);
-  return launch_fp8<SWIGLU, 1, 128>(fp, most_tiles, dev, info.sm_count, s);
+  if (rc != 0) return rc;
+  const int sms = info.sm_count;
+  if (v.cg == 2) return launch_fp8<SWIGLU, 2, 256, 128, 1>(fp, most_tiles, dev, sms, s);
+  if (v.rows == 32) {
+    if (v.bn == 128) {
+      switch (v.split) {
+        case 8:
+          return launch_fp8<SWIGLU, 1, 128, 32, 8>(fp, most_tiles, dev, sms, s);
+        case 4:
+          return launch_fp8<SWIGLU, 1, 128, 32, 4>(fp, most_tiles, dev, sms, s);
+        case 2:
+          return launch_fp8<SWIGLU, 1, 128, 32, 2>(fp, most_tiles, dev, sms, s);
+        default:
+          return launch_fp8<SWIGLU, 1, 128, 32, 1>(fp, most_tiles, dev, sms, s);
+      }
+    }
+    switch (v.split) {
+      case 8:
+        return launch_fp8<SWIGLU, 1, 64, 32, 8>(fp, most_tiles, dev, sms, s);
+      case 4:
+        return launch_fp8<SWIGLU, 1, 64, 32, 4>(fp, most_tiles, dev, sms, s);
+      case 2:
+        return launch_fp8<SWIGLU, 1, 64, 32, 2>(fp, most_tiles, dev, sms, s);
+      default:
+        return launch_fp8<SWIGLU, 1, 64, 32, 1>(fp, most_tiles, dev, sms, s);
+    }
+  }
+  if (v.bn == 256) return launch_fp8<SWIGLU, 1, 256, 128, 1>(fp, most_tiles, dev, sms, s);
+  return launch_fp8<SWIGLU, 1, 128, 128, 1>(fp, most_tiles, dev, sms, s);
 }
 
 template <bool SWIGLU>

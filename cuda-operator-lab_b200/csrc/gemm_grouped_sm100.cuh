@@ -37,8 +37,9 @@ namespace sm100 {
 enum GroupedMode : int { kForward = 0, kGradX = 1, kGradW = 2 };
 
 struct __align__(64) GroupedParams {
-  CUtensorMap map_a;
-  CUtensorMap map_b;
+  CUtensorMap map_a;    // boxes of 128 rows (kGradW: 64)
+  CUtensorMap map_a32;  // the same in boxes of 32 rows (single CTAs)
+  CUtensorMap map_b;    // boxes of b_box_rows() rows (gradients: 64)
   const int* offsets;
   __nv_bfloat16* out;
   unsigned* status;
@@ -55,12 +56,20 @@ struct __align__(64) GroupedParams {
 constexpr uint32_t kGroupedTableBytes = 4352;  // prefix table of kMaxGroups + 1 ints
 static_assert(kGroupedTableBytes >= (kMaxGroups + 1) * 4, "table size");
 
-template <int CG, int BN>
+// B is loaded in two boxes where gate and up rows or two CTAs share it.
+constexpr int b_box_rows(bool swiglu, int cg, int bn) { return swiglu || cg == 2 ? bn / 2 : bn; }
+
+// ROWS = 32: tiles of at most 32 rows, for products whose time is reading w.
+// Only those rows of A are loaded and kept (the MMA's other 96 rows read
+// whatever lies behind them; what they add up is not stored), which leaves the
+// ring to w.
+template <int CG, int BN, int ROWS>
 struct GroupedCfg {
   static_assert(BN == 64 || BN == 128 || BN == 256, "tile width");
   static_assert(CG == 1 || CG == 2, "CTAs of a tile");
-  static constexpr int kTileRows = kBlockM * CG;
-  static constexpr uint32_t kABytes = kBlockM * kBlockK * 2;
+  static_assert(ROWS == kBlockM || (ROWS == 32 && CG == 1), "rows of a tile");
+  static constexpr int kTileRows = ROWS * CG;
+  static constexpr uint32_t kABytes = ROWS * kBlockK * 2;
   static constexpr uint32_t kBBytes = BN / CG * kBlockK * 2;
   static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
   static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : 2;  // k-blocks a stage
@@ -138,9 +147,9 @@ __device__ __forceinline__ bool elect_one() {
 // Bounded wait of a whole converged warp (mbar_wait is one thread's).  All
 // lanes poll with one instruction, read one flag and count alike, so that they
 // leave together; a count needs no registers for clocks, of which the e4m3
-// kernel's readers have none to spare.  2^24 polls are a quarter of a second
-// at the least.
-constexpr uint32_t kWarpWaitPolls = 1u << 24;
+// kernel's readers have none to spare.  2^20 polls are ~20 ms at the least,
+// thousands of times what any of these waits takes.
+constexpr uint32_t kWarpWaitPolls = 1u << 20;
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
@@ -180,17 +189,29 @@ struct GroupedTile {
   int begin;    // the group's rows
   int end;
   int k_blocks;
+  int first_k;  // k-block that the sum starts with (few_rows_first_k)
 };
 
-template <int MODE, bool SWIGLU, int CG, int BN>
+// Tiles of few rows stream w from DRAM.  Started together, they would read the
+// same columns of all their rows, addresses that agree in their low bits, and
+// crowd on few channels; so each tile's sum starts at another (even, its stages
+// read pairs) k-block and wraps around.  256 rows over 64 experts, gate/up 2048
+// x 4096 in bf16: 157 -> 136 us.  It depends on the expert and the columns
+// alone, so a row's result does not depend on the other rows.
+__device__ __forceinline__ int few_rows_first_k(int group, int n_block, int num_n, int k_blocks) {
+  const unsigned tile = static_cast<unsigned>(group) * num_n + n_block;
+  return static_cast<int>(2u * (tile * 5u % ((k_blocks + 1u) / 2u)));
+}
+
+template <int MODE, bool SWIGLU, int CG, int BN, int ROWS>
 __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, const int* prefix,
                                                     int tile, int rank) {
-  using Cfg = GroupedCfg<CG, BN>;
+  constexpr int kTileRows = ROWS * CG;
   GroupedTile t;
   TileCoords c;
   if constexpr (MODE == kGradW) {
     // every group has the same tiles
-    const int m_blocks = (p.out_rows + Cfg::kTileRows - 1) / Cfg::kTileRows;
+    const int m_blocks = (p.out_rows + kTileRows - 1) / kTileRows;
     const int per_group = m_blocks * p.num_n_blocks;
     c.group = tile / per_group;
     const int local = tile - c.group * per_group;
@@ -203,9 +224,10 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
   t.group = c.group;
   t.begin = r.begin;
   t.end = r.end;
-  t.a_row = (MODE == kGradW ? 0 : r.begin) + c.m * Cfg::kTileRows + rank * kBlockM;
+  t.a_row = (MODE == kGradW ? 0 : r.begin) + c.m * kTileRows + rank * ROWS;
   t.col = c.n * (SWIGLU ? BN / 2 : BN);
   t.k_blocks = MODE == kGradW ? (r.end - r.begin + kBlockK - 1) / kBlockK : p.num_k_blocks;
+  t.first_k = ROWS == 32 ? few_rows_first_k(c.group, c.n, p.num_n_blocks, p.num_k_blocks) : 0;
   return t;
 }
 
@@ -289,20 +311,18 @@ __device__ __forceinline__ void store_rows64(const GroupedParams& p, std::size_t
   }
 }
 
-template <int MODE, bool SWIGLU, int CG, int BN>
+template <int MODE, bool SWIGLU, int CG, int BN, int ROWS>
 __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     grouped_bf16_kernel(const __grid_constant__ GroupedParams p) {
-  using Cfg = GroupedCfg<CG, BN>;
+  using Cfg = GroupedCfg<CG, BN, ROWS>;
+  static_assert(MODE != kGradW || ROWS == kBlockM, "rows of w are not ragged");
   static_assert(MODE == kForward || !SWIGLU, "SwiGLU is a forward epilogue");
   constexpr int kStages = Cfg::kStages;
   constexpr int kKps = Cfg::kKps;
-  constexpr uint32_t kIdesc = idesc_bf16_f32(Cfg::kTileRows, BN) |
+  constexpr uint32_t kIdesc = idesc_bf16_f32(kBlockM * CG, BN) |
                               (MODE == kGradW ? kIdescAMnMajor : 0u) |
                               (MODE != kForward ? kIdescBMnMajor : 0u);
   constexpr uint32_t kChunkBytes = 64 * kBlockK * 2;  // 64 columns x 64 rows
-  // Forward with single CTAs serves few rows a group: A is loaded 32 rows at a
-  // time, only those the group has.
-  constexpr int kABoxRows = MODE == kGradW ? kBlockK : (CG == 1 ? 32 : kBlockM);
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -374,33 +394,34 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   }
 
   if (warp == 0) {
-    if (lane == 0) {
-      // ---------------- TMA producer
+    // ---------------- TMA producer: the whole warp keeps the loop's state, so
+    // that addresses and coordinates stay in uniform registers; one lane issues
+    if (elect_one()) {
       prefetch_tmap(&p.map_a);
       prefetch_tmap(&p.map_b);
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t issued_mask = 0;
-      uint32_t issued_phase = 0;
-      int filled = 0;
-      bool ok = true;
-      for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
-        int a_boxes = kBlockM / kABoxRows;
-        if constexpr (MODE != kGradW && CG == 1) {
-          a_boxes = min(a_boxes, (t.end - t.a_row + kABoxRows - 1) / kABoxRows);
+    }
+    __syncwarp();
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t issued_mask = 0;
+    uint32_t issued_phase = 0;
+    int filled = 0;
+    bool ok = true;
+    for (int tile = worker; ok && tile < num_tiles; tile += workers) {
+      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+      // Single CTAs load A 32 rows at a time where the group ends early.
+      const int rows = min(ROWS, (t.end - t.a_row + 31) & ~31);
+      const bool whole = MODE == kGradW || CG == 2 || rows == kBlockM;
+      const bool ragged = MODE == kGradW && ragged_rows(t) != 0;
+      for (int kb = 0; kb < t.k_blocks; kb += kKps) {
+        if (filled >= kStages && !warp_wait(smem_u32(empty_bar + stage), phase ^ 1u, abort_flag)) {
+          if (lane == 0) fail(kStatusProducer);
+          ok = false;
+          break;
         }
-        const bool ragged = MODE == kGradW && ragged_rows(t) != 0;
-        for (int kb = 0; kb < t.k_blocks; kb += kKps) {
-          if (filled >= kStages && !mbar_wait(smem_u32(empty_bar + stage), phase ^ 1u, abort_flag)) {
-            fail(kStatusProducer);
-            ok = false;
-            break;
-          }
-          const int nk = min(kKps, t.k_blocks - kb);
-          const uint32_t a_bytes =
-              MODE != kGradW && CG == 1 ? a_boxes * kABoxRows * 128u : Cfg::kABytes;
-          const uint32_t bytes = nk * (a_bytes + Cfg::kBBytes);
+        const int nk = min(kKps, t.k_blocks - kb);
+        if (elect_one()) {
+          const uint32_t bytes = nk * ((whole ? Cfg::kABytes : rows * 128u) + Cfg::kBBytes);
           const uint32_t fb_local = smem_u32(full_bar + stage);
           uint32_t fb = fb_local;
           if constexpr (CG == 2) fb = map_to_cta(fb_local, 0);
@@ -420,25 +441,29 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
             if (j >= nk) break;
             const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
             const uint32_t sb = sa + Cfg::kABytes;
-            const int kc = (kb + j) * kBlockK;
+            int kc = kb + j + t.first_k;
+            if (ROWS == 32 && kc >= t.k_blocks) kc -= t.k_blocks;
+            kc *= kBlockK;
             if constexpr (MODE == kGradW) {
 #pragma unroll
               for (int i = 0; i < kBlockM / 64; ++i) {
                 grouped_load_2d<CG>(sa + i * kChunkBytes, &p.map_a, fb, t.a_row + 64 * i,
                                     t.begin + kc);
               }
+            } else if (whole) {
+              grouped_load_2d<CG>(sa, &p.map_a, fb, kc, t.a_row);
             } else {
-              for (int i = 0; i < a_boxes; ++i) {
-                grouped_load_2d<CG>(sa + i * (kABoxRows * 128), &p.map_a, fb, kc,
-                                    t.a_row + i * kABoxRows);
+              for (int r = 0; r < rows; r += 32) {
+                grouped_load_2d<CG>(sa + r * 128, &p.map_a32, fb, kc, t.a_row + r);
               }
             }
             if constexpr (MODE == kForward) {
               // half h of B: rows n0 + h BN/2 of w, or gate (0) and up (1) rows
+              constexpr int kBoxRows = b_box_rows(SWIGLU, CG, BN);
 #pragma unroll
-              for (int i = 0; i < 2 / CG; ++i) {
+              for (int i = 0; i < BN / CG / kBoxRows; ++i) {
                 const int h = CG == 2 ? rank : i;
-                grouped_load_3d<CG>(sb + i * (BN / 2 * 128), &p.map_b, fb, kc,
+                grouped_load_3d<CG>(sb + i * (kBoxRows * 128), &p.map_b, fb, kc,
                                     t.col + h * (SWIGLU ? p.up_offset : BN / 2), t.group);
               }
             } else {
@@ -453,27 +478,28 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
               }
             }
           }
-          if (filled < kStages) ++filled;
-          issued_mask |= 1u << stage;
-          issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+        }
+        __syncwarp();
+        if (filled < kStages) ++filled;
+        issued_mask |= 1u << stage;
+        issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
         }
       }
-      if (!ok || *abort_flag) {
-        if (leader) {
-          for (int s = 0; s < kStages; ++s) {
-            if ((issued_mask & (1u << s)) &&
-                !mbar_wait_drain(smem_u32(full_bar + s), (issued_phase >> s) & 1u)) {
-              atomicOr(p.status, kStatusDrain);
-            }
+    }
+    if (lane == 0 && (!ok || *abort_flag)) {
+      if (leader) {
+        for (int s = 0; s < kStages; ++s) {
+          if ((issued_mask & (1u << s)) &&
+              !mbar_wait_drain(smem_u32(full_bar + s), (issued_phase >> s) & 1u)) {
+            atomicOr(p.status, kStatusDrain);
           }
-        } else {
-          // CTA 1 cannot observe CTA 0's barriers: give its copies time to land.
-          for (int i = 0; i < 200; ++i) __nanosleep(1000);
         }
+      } else {
+        // CTA 1 cannot observe CTA 0's barriers: give its copies time to land.
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
       }
     }
   } else if (warp == 1) {
@@ -486,7 +512,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       bool ok = true;
       bool issued_any = false;
       for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
+        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
         if (MODE == kGradW && t.k_blocks == 0) continue;  // zeros, stored without a sum
         const int acc = local & 1;
         if (!warp_wait(smem_u32(tempty_bar + acc), ((local >> 1) & 1) ^ 1u, abort_flag)) {
@@ -556,7 +582,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       int stage = 0;  // slot of this tile's first stage
       uint32_t tail_phase = 0;  // bit s: parity of tail_bar[s]'s next completion
       for (int tile = worker; tile < num_tiles; tile += workers) {
-        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
+        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
         const int stages = (t.k_blocks + kKps - 1) / kKps;
         const int first = ragged_rows(t);
         if (first != 0) {
@@ -599,10 +625,12 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     const int half = (warp - 4) >> 2;
     int local = 0;
     for (int tile = worker; tile < num_tiles; tile += workers) {
-      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN>(p, prefix, tile, rank);
+      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
       const int row0 = t.a_row + q * 32;
       // rows of this warp to store; none: they all lie behind the group's last
-      const int valid = min((MODE == kGradW ? p.out_rows : t.end) - row0, 32);
+      const int valid = ROWS == 32 && q != 0
+                            ? 0
+                            : min((MODE == kGradW ? p.out_rows : t.end) - row0, 32);
       const std::size_t out_row =
           MODE == kGradW ? static_cast<std::size_t>(t.group) * p.out_rows + row0 : row0;
       // output columns of the tile and of this warp
@@ -648,6 +676,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
           } else {
 #pragma unroll
             for (int h = 0; h < kRun; h += 32) {
+              static_assert(SWIGLU || kRun >= 32, "columns of a run");
               uint32_t a[32];
               tmem_ld32(t_row + c + h, a);
 #pragma unroll

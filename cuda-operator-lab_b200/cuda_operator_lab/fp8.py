@@ -18,6 +18,7 @@ boundaries, elsewhere on a much slower CUDA-core kernel.
 from __future__ import annotations
 
 import torch
+from torch._C import _cuda_getDevice as _current_device
 
 from .bindings import _call, _ptr, _stream
 
@@ -37,17 +38,27 @@ def _blocks(size: int) -> int:
     return -(-size // BLOCK)
 
 
+def _placed(*tensors: torch.Tensor) -> bool:
+    """Whether all are contiguous CUDA tensors of one device."""
+    device = tensors[0].get_device()  # -1 off the GPU
+    if device < 0:
+        return False
+    for t in tensors:
+        if not t.is_contiguous() or t.get_device() != device:
+            return False
+    return True
+
+
 def _check_placement(what: str, *tensors: torch.Tensor) -> None:
-    """Contiguous CUDA tensors of one device."""
+    if _placed(*tensors):
+        return
     for t in tensors:
         if not t.is_contiguous():
             raise ValueError(f"all {what} tensors must be contiguous")
     for t in tensors:
         if not t.is_cuda:
             raise ValueError(f"{what} tensors must be CUDA tensors")
-    for t in tensors:
-        if t.device != tensors[0].device:
-            raise ValueError(f"{what} tensors must be on one device")
+    raise ValueError(f"{what} tensors must be on one device")
 
 
 def _check_sizes(what: str, *sizes: int) -> None:
@@ -58,7 +69,7 @@ def _check_sizes(what: str, *sizes: int) -> None:
 
 def _launch(symbol: str, on: torch.Tensor, *args) -> None:
     """One library call on the current stream of ``on``'s device."""
-    if on.get_device() == torch.cuda.current_device():
+    if on.get_device() == _current_device():
         _call(symbol, *args, _stream(on))
     else:
         with torch.cuda.device(on.device):
@@ -68,12 +79,19 @@ def _launch(symbol: str, on: torch.Tensor, *args) -> None:
 # ---------------------------------------------------------------- quantisation
 
 
-def _source_suffix(what: str, x: torch.Tensor) -> str:
-    if x.dtype == torch.bfloat16:
-        return "bf16"
-    if x.dtype == torch.float32:
-        return "f32"
-    raise TypeError(f"{what} expects a bfloat16 or float32 input")
+# The calls are host-bound at small sizes, so an operator's checks are first one
+# expression that reads each attribute once; where it does not hold, the checks
+# run one by one and raise.  The allocating forms do not check what they made.
+
+_ROWS = {torch.bfloat16: "cuda_operator_quantize_fp8_block128_bf16",
+         torch.float32: "cuda_operator_quantize_fp8_block128_f32"}
+_TILES = {torch.bfloat16: "cuda_operator_quantize_fp8_block128_weight_bf16",
+          torch.float32: "cuda_operator_quantize_fp8_block128_weight_f32"}
+
+
+def _check_source(what: str, x: torch.Tensor) -> None:
+    if x.dtype not in _ROWS:
+        raise TypeError(f"{what} expects a bfloat16 or float32 input")
 
 
 def _check_quantized(what: str, x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor,
@@ -86,34 +104,49 @@ def _check_quantized(what: str, x: torch.Tensor, q: torch.Tensor, scale: torch.T
         raise TypeError(f"{what} writes float8_e4m3fn values and float32 scales")
 
 
+def _check_rows(x: torch.Tensor) -> tuple[int, int]:
+    if x.ndim != 2:
+        raise ValueError("x must be 2-D")
+    _check_source("FP8 quantize", x)
+    m, k = x.shape
+    _check_sizes("FP8 quantize", m, k)
+    return m, k
+
+
 def quantize_fp8_block128_into(x: torch.Tensor, q: torch.Tensor,
                                scale: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Rows [M, K] (bf16 or fp32) to e4m3 [M, K] and fp32 scales [M, ceil(K/128)]."""
-    what = "FP8 quantize"
-    if x.ndim != 2:
-        raise ValueError("x must be 2-D")
-    suffix = _source_suffix(what, x)
-    m, k = x.shape
-    _check_quantized(what, x, q, scale, (m, _blocks(k)))
-    _check_sizes(what, m, k)
-    _check_placement(what, x, q, scale)
+    m, k = _check_rows(x)
+    _check_quantized("FP8 quantize", x, q, scale, (m, _blocks(k)))
+    _check_placement("FP8 quantize", x, q, scale)
     if m and k:
-        _launch(f"cuda_operator_quantize_fp8_block128_{suffix}", x, _ptr(x), _ptr(q), _ptr(scale),
-                m, k)
+        _launch(_ROWS[x.dtype], x, _ptr(x), _ptr(q), _ptr(scale), m, k)
     return q, scale
 
 
 def quantize_fp8_block128(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Allocating form of :func:`quantize_fp8_block128_into`: ``(q, scale)``."""
-    if x.ndim != 2:
-        raise ValueError("x must be 2-D")
-    q = torch.empty(x.shape, device=x.device, dtype=_E4M3)
-    scale = torch.empty((x.shape[0], _blocks(x.shape[1])), device=x.device, dtype=torch.float32)
-    return quantize_fp8_block128_into(x, q, scale)
+    m, k = _check_rows(x)
+    _check_placement("FP8 quantize", x)
+    q = torch.empty_like(x, dtype=_E4M3)
+    scale = x.new_empty((m, _blocks(k)), dtype=torch.float32)
+    if m and k:
+        _launch(_ROWS[x.dtype], x, _ptr(x), _ptr(q), _ptr(scale), m, k)
+    return q, scale
 
 
 def _weight_scale_shape(shape: torch.Size) -> tuple[int, ...]:
     return (*shape[:-2], _blocks(shape[-2]), _blocks(shape[-1]))
+
+
+def _check_weight(weight: torch.Tensor) -> tuple[int, int, int]:
+    if weight.ndim not in (2, 3):
+        raise ValueError("weight must be 2-D or 3-D")
+    _check_source("FP8 weight quantize", weight)
+    n, k = weight.shape[-2:]
+    experts = weight.shape[0] if weight.ndim == 3 else 1
+    _check_sizes("FP8 weight quantize", n, k, experts * _blocks(n) * _blocks(k))
+    return experts, n, k
 
 
 def quantize_fp8_block128_weight_into(weight: torch.Tensor, q: torch.Tensor,
@@ -123,28 +156,23 @@ def quantize_fp8_block128_weight_into(weight: torch.Tensor, q: torch.Tensor,
     ``scale`` is [ceil(N/128), ceil(K/128)], with E in front where the weight has it.
     """
     what = "FP8 weight quantize"
-    if weight.ndim not in (2, 3):
-        raise ValueError("weight must be 2-D or 3-D")
-    suffix = _source_suffix(what, weight)
+    experts, n, k = _check_weight(weight)
     _check_quantized(what, weight, q, scale, _weight_scale_shape(weight.shape))
-    n, k = weight.shape[-2:]
-    experts = weight.shape[0] if weight.ndim == 3 else 1
-    _check_sizes(what, n, k, experts * _blocks(n) * _blocks(k))
     _check_placement(what, weight, q, scale)
-    if weight.numel():
-        _launch(f"cuda_operator_quantize_fp8_block128_weight_{suffix}", weight, _ptr(weight),
-                _ptr(q), _ptr(scale), experts, n, k)
+    if experts and n and k:
+        _launch(_TILES[weight.dtype], weight, _ptr(weight), _ptr(q), _ptr(scale), experts, n, k)
     return q, scale
 
 
 def quantize_fp8_block128_weight(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Allocating form of :func:`quantize_fp8_block128_weight_into`: ``(q, scale)``."""
-    if weight.ndim not in (2, 3):
-        raise ValueError("weight must be 2-D or 3-D")
-    q = torch.empty(weight.shape, device=weight.device, dtype=_E4M3)
-    scale = torch.empty(_weight_scale_shape(weight.shape), device=weight.device,
-                        dtype=torch.float32)
-    return quantize_fp8_block128_weight_into(weight, q, scale)
+    experts, n, k = _check_weight(weight)
+    _check_placement("FP8 weight quantize", weight)
+    q = torch.empty_like(weight, dtype=_E4M3)
+    scale = weight.new_empty(_weight_scale_shape(weight.shape), dtype=torch.float32)
+    if experts and n and k:
+        _launch(_TILES[weight.dtype], weight, _ptr(weight), _ptr(q), _ptr(scale), experts, n, k)
+    return q, scale
 
 
 # ---------------------------------------------------------------- products
@@ -152,40 +180,54 @@ def quantize_fp8_block128_weight(weight: torch.Tensor) -> tuple[torch.Tensor, to
 
 def _check_fp8_operands(what: str, x_fp8: torch.Tensor, x_scale: torch.Tensor,
                         weight_fp8: torch.Tensor, weight_scale: torch.Tensor,
-                        out: torch.Tensor, swiglu: bool) -> tuple[int, int, int]:
+                        swiglu: bool) -> tuple[int, int, int]:
     """Shapes and types shared by the dense and the grouped products; returns (rows, k, n)."""
     m, k = x_fp8.shape
-    w_rows = weight_fp8.shape[-2]
-    if weight_fp8.shape[-1] != k:
+    w_shape = weight_fp8.shape
+    w_rows = w_shape[-2]
+    if (w_shape[-1] == k and k > 0 and not (swiglu and w_rows % (2 * BLOCK))
+            and x_scale.shape == (m, _blocks(k))
+            and weight_scale.shape == (*w_shape[:-2], _blocks(w_rows), _blocks(k))
+            and x_fp8.dtype is _E4M3 and weight_fp8.dtype is _E4M3
+            and x_scale.dtype is torch.float32 and weight_scale.dtype is torch.float32
+            and m <= _MAX_SIZE and k <= _MAX_SIZE and w_rows <= _MAX_SIZE):
+        return m, k, w_rows // 2 if swiglu else w_rows
+    if w_shape[-1] != k:
         raise ValueError("x.shape[1] must equal the weight's last dimension")
     if k == 0:
         raise ValueError(f"{what} requires k > 0")
     if swiglu and w_rows % (2 * BLOCK):
         raise ValueError(f"{what} needs gate and up rows in whole blocks of {BLOCK}")
-    n = w_rows // 2 if swiglu else w_rows
     if x_scale.shape != (m, _blocks(k)):
         raise ValueError(f"x scale shape must be {(m, _blocks(k))}")
-    if weight_scale.shape != _weight_scale_shape(weight_fp8.shape):
-        raise ValueError(f"weight scale shape must be {_weight_scale_shape(weight_fp8.shape)}")
-    if out.shape != (m, n):
-        raise ValueError(f"output shape must be {(m, n)}")
+    if weight_scale.shape != _weight_scale_shape(w_shape):
+        raise ValueError(f"weight scale shape must be {_weight_scale_shape(w_shape)}")
     if x_fp8.dtype != _E4M3 or weight_fp8.dtype != _E4M3:
         raise TypeError(f"{what} expects float8_e4m3fn x and weight")
     if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
         raise TypeError(f"{what} expects float32 scales")
+    raise ValueError(f"{what} sizes must be at most {_MAX_SIZE}")
+
+
+def _check_output(what: str, out: torch.Tensor, shape: tuple[int, ...]) -> None:
+    if out.shape != shape:
+        raise ValueError(f"output shape must be {shape}")
     if out.dtype != torch.bfloat16:
         raise TypeError(f"{what} expects a bfloat16 output")
-    _check_sizes(what, m, k, w_rows)
-    return m, k, n
 
 
-def _gemm_into(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
-               weight_scale: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+def _gemm(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
+          weight_scale: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     what = "FP8 GEMM SwiGLU" if swiglu else "FP8 GEMM"
     if x_fp8.ndim != 2 or weight_fp8.ndim != 2:
         raise ValueError("x and weight must be 2-D")
-    m, k, n = _check_fp8_operands(what, x_fp8, x_scale, weight_fp8, weight_scale, out, swiglu)
-    _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, out)
+    m, k, n = _check_fp8_operands(what, x_fp8, x_scale, weight_fp8, weight_scale, swiglu)
+    if out is None:
+        _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale)
+        out = x_fp8.new_empty((m, n), dtype=torch.bfloat16)
+    else:
+        _check_output(what, out, (m, n))
+        _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, out)
     if m and n:
         symbol = "cuda_operator_gemm_swiglu_fp8_block128" if swiglu else "cuda_operator_gemm_fp8_block128"
         _launch(symbol, x_fp8, _ptr(x_fp8), _ptr(x_scale), _ptr(weight_fp8), _ptr(weight_scale),
@@ -196,17 +238,13 @@ def _gemm_into(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_
 def gemm_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
                            weight_scale: torch.Tensor, out_bf16: torch.Tensor) -> torch.Tensor:
     """bf16(x @ W.T) of block-scaled e4m3 x [M, K] and W [N, K], products and sums in fp32."""
-    return _gemm_into(False, x_fp8, x_scale, weight_fp8, weight_scale, out_bf16)
+    return _gemm(False, x_fp8, x_scale, weight_fp8, weight_scale, out_bf16)
 
 
 def gemm_fp8_block128(x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
                       weight_scale: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_fp8_block128_into`."""
-    if x_fp8.ndim != 2 or weight_fp8.ndim != 2:
-        raise ValueError("x and weight must be 2-D")
-    out = torch.empty((x_fp8.shape[0], weight_fp8.shape[0]), device=x_fp8.device,
-                      dtype=torch.bfloat16)
-    return gemm_fp8_block128_into(x_fp8, x_scale, weight_fp8, weight_scale, out)
+    return _gemm(False, x_fp8, x_scale, weight_fp8, weight_scale, None)
 
 
 def gemm_swiglu_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Tensor,
@@ -216,15 +254,11 @@ def gemm_swiglu_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Tensor,
 
     N must be a multiple of 128, so that no tile of scales spans gate and up rows.
     """
-    return _gemm_into(True, x_fp8, x_scale, packed_weight_fp8, weight_scale, out_bf16)
+    return _gemm(True, x_fp8, x_scale, packed_weight_fp8, weight_scale, out_bf16)
 
 
 def gemm_swiglu_fp8_block128(x_fp8: torch.Tensor, x_scale: torch.Tensor,
                              packed_weight_fp8: torch.Tensor,
                              weight_scale: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_swiglu_fp8_block128_into`."""
-    if x_fp8.ndim != 2 or packed_weight_fp8.ndim != 2:
-        raise ValueError("x and weight must be 2-D")
-    out = torch.empty((x_fp8.shape[0], packed_weight_fp8.shape[0] // 2), device=x_fp8.device,
-                      dtype=torch.bfloat16)
-    return gemm_swiglu_fp8_block128_into(x_fp8, x_scale, packed_weight_fp8, weight_scale, out)
+    return _gemm(True, x_fp8, x_scale, packed_weight_fp8, weight_scale, None)

@@ -24,7 +24,8 @@ from __future__ import annotations
 import torch
 
 from .bindings import _ptr
-from .fp8 import _check_fp8_operands, _check_placement, _check_sizes, _launch
+from .fp8 import (_check_fp8_operands, _check_output, _check_placement, _check_sizes, _launch,
+                  _MAX_SIZE)
 
 __all__ = [
     "gemm_grouped_bf16", "gemm_grouped_bf16_into",
@@ -63,25 +64,41 @@ def _check_ranks(x: torch.Tensor, weight: torch.Tensor) -> None:
 # ---------------------------------------------------------------- bf16
 
 
-def _forward_into(swiglu: bool, x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
-                  out: torch.Tensor) -> torch.Tensor:
-    what = "grouped GEMM SwiGLU" if swiglu else "grouped GEMM"
+def _check_forward(what: str, swiglu: bool, x: torch.Tensor, weight: torch.Tensor,
+                   offsets: torch.Tensor) -> tuple[int, int, int, int]:
+    """Checks of all but the output and the placement; returns (t, k, n, experts)."""
     _check_ranks(x, weight)
     t, k = x.shape
-    experts, w_rows, _ = weight.shape
-    if weight.shape[2] != k:
+    experts, w_rows, w_cols = weight.shape
+    n = w_rows // 2 if swiglu else w_rows
+    if (w_cols == k and k > 0 and not (swiglu and w_rows % 2)
+            and offsets.shape == (experts + 1,) and offsets.dtype is torch.int32
+            and x.dtype is torch.bfloat16 and weight.dtype is torch.bfloat16
+            and experts <= MAX_EXPERTS and t <= _MAX_SIZE and k <= _MAX_SIZE
+            and w_rows <= _MAX_SIZE):
+        return t, k, n, experts
+    if w_cols != k:
         raise ValueError("x.shape[1] must equal weight.shape[2]")
     if k == 0:
         raise ValueError(f"{what} requires k > 0")
     if swiglu and w_rows % 2:
         raise ValueError("packed weight must have an even number of rows")
-    n = w_rows // 2 if swiglu else w_rows
-    if out.shape != (t, n):
-        raise ValueError(f"output shape must be {(t, n)}")
     _check_offsets(what, offsets, experts)
-    _check_bf16(what, x, weight, out)
+    _check_bf16(what, x, weight)
     _check_sizes(what, t, k, w_rows)
-    _check_placement(what, x, weight, offsets, out)
+    raise AssertionError("unreachable")
+
+
+def _forward(swiglu: bool, x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
+             out: torch.Tensor | None) -> torch.Tensor:
+    what = "grouped GEMM SwiGLU" if swiglu else "grouped GEMM"
+    t, k, n, experts = _check_forward(what, swiglu, x, weight, offsets)
+    if out is None:
+        _check_placement(what, x, weight, offsets)
+        out = x.new_empty((t, n))
+    else:
+        _check_output(what, out, (t, n))
+        _check_placement(what, x, weight, offsets, out)
     if t and n and experts:
         symbol = "cuda_operator_gemm_grouped_swiglu_bf16" if swiglu else "cuda_operator_gemm_grouped_bf16"
         _launch(symbol, x, _ptr(x), _ptr(weight), _ptr(offsets), _ptr(out), t, k, n, experts)
@@ -91,57 +108,50 @@ def _forward_into(swiglu: bool, x: torch.Tensor, weight: torch.Tensor, offsets: 
 def gemm_grouped_bf16_into(x_bf16: torch.Tensor, weight_bf16: torch.Tensor, offsets: torch.Tensor,
                            out_bf16: torch.Tensor) -> torch.Tensor:
     """bf16(x[r] @ W[e].T) for the rows r of each expert e; x [T, K], W [E, N, K], out [T, N]."""
-    return _forward_into(False, x_bf16, weight_bf16, offsets, out_bf16)
+    return _forward(False, x_bf16, weight_bf16, offsets, out_bf16)
 
 
 def gemm_grouped_bf16(x_bf16: torch.Tensor, weight_bf16: torch.Tensor,
                       offsets: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_grouped_bf16_into`."""
-    _check_ranks(x_bf16, weight_bf16)
-    out = torch.empty((x_bf16.shape[0], weight_bf16.shape[1]), device=x_bf16.device,
-                      dtype=torch.bfloat16)
-    return gemm_grouped_bf16_into(x_bf16, weight_bf16, offsets, out)
+    return _forward(False, x_bf16, weight_bf16, offsets, None)
 
 
 def gemm_grouped_swiglu_bf16_into(x_bf16: torch.Tensor, packed_weight_bf16: torch.Tensor,
                                   offsets: torch.Tensor, out_bf16: torch.Tensor) -> torch.Tensor:
     """bf16(silu(x[r] @ Wg[e].T) * (x[r] @ Wu[e].T)); packed weight [E, 2N, K], gate rows first."""
-    return _forward_into(True, x_bf16, packed_weight_bf16, offsets, out_bf16)
+    return _forward(True, x_bf16, packed_weight_bf16, offsets, out_bf16)
 
 
 def gemm_grouped_swiglu_bf16(x_bf16: torch.Tensor, packed_weight_bf16: torch.Tensor,
                              offsets: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_grouped_swiglu_bf16_into`."""
-    _check_ranks(x_bf16, packed_weight_bf16)
-    out = torch.empty((x_bf16.shape[0], packed_weight_bf16.shape[1] // 2), device=x_bf16.device,
-                      dtype=torch.bfloat16)
-    return gemm_grouped_swiglu_bf16_into(x_bf16, packed_weight_bf16, offsets, out)
+    return _forward(True, x_bf16, packed_weight_bf16, offsets, None)
 
 
 # ---------------------------------------------------------------- bf16 gradients
 
 
-def _check_grad_input(grad: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
-                      out: torch.Tensor) -> None:
-    what = "grouped GEMM gradient"
+_GRAD = "grouped GEMM gradient"
+
+
+def _check_grad_input(grad: torch.Tensor, weight: torch.Tensor,
+                      offsets: torch.Tensor) -> tuple[int, int, int, int]:
     _check_ranks(grad, weight)
     t, n = grad.shape
-    experts, _, k = weight.shape
-    if weight.shape[1] != n:
+    experts, w_rows, k = weight.shape
+    if w_rows != n:
         raise ValueError("grad.shape[1] must equal weight.shape[1]")
     if n == 0:
-        raise ValueError(f"{what} requires n > 0")
-    if out.shape != (t, k):
-        raise ValueError(f"output shape must be {(t, k)}")
-    _check_offsets(what, offsets, experts)
-    _check_bf16(what, grad, weight, out)
-    _check_sizes(what, t, k, n)
+        raise ValueError(f"{_GRAD} requires n > 0")
+    _check_offsets(_GRAD, offsets, experts)
+    _check_bf16(_GRAD, grad, weight)
+    _check_sizes(_GRAD, t, k, n)
+    return t, k, n, experts
 
 
 def _run_grad_input(grad: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
-                    out: torch.Tensor) -> torch.Tensor:
-    t, n = grad.shape
-    experts, _, k = weight.shape
+                    out: torch.Tensor, t: int, k: int, n: int, experts: int) -> torch.Tensor:
     if t and k and experts:
         _launch("cuda_operator_gemm_grouped_bf16_grad_input", grad, _ptr(grad), _ptr(weight),
                 _ptr(offsets), _ptr(out), t, k, n, experts)
@@ -152,43 +162,43 @@ def gemm_grouped_bf16_grad_input_into(grad_bf16: torch.Tensor, weight_bf16: torc
                                       offsets: torch.Tensor,
                                       grad_input_bf16: torch.Tensor) -> torch.Tensor:
     """Gradient of :func:`gemm_grouped_bf16` by x: bf16(grad[r] @ W[e]); grad [T, N], out [T, K]."""
-    _check_grad_input(grad_bf16, weight_bf16, offsets, grad_input_bf16)
-    _check_placement("grouped GEMM gradient", grad_bf16, weight_bf16, offsets, grad_input_bf16)
-    return _run_grad_input(grad_bf16, weight_bf16, offsets, grad_input_bf16)
+    t, k, n, experts = _check_grad_input(grad_bf16, weight_bf16, offsets)
+    _check_output(_GRAD, grad_input_bf16, (t, k))
+    _check_placement(_GRAD, grad_bf16, weight_bf16, offsets, grad_input_bf16)
+    return _run_grad_input(grad_bf16, weight_bf16, offsets, grad_input_bf16, t, k, n, experts)
 
 
 def gemm_grouped_bf16_grad_input(grad_bf16: torch.Tensor, weight_bf16: torch.Tensor,
                                  offsets: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_grouped_bf16_grad_input_into`."""
-    _check_ranks(grad_bf16, weight_bf16)
-    out = torch.empty((grad_bf16.shape[0], weight_bf16.shape[2]), device=grad_bf16.device,
-                      dtype=torch.bfloat16)
-    return gemm_grouped_bf16_grad_input_into(grad_bf16, weight_bf16, offsets, out)
+    t, k, n, experts = _check_grad_input(grad_bf16, weight_bf16, offsets)
+    _check_placement(_GRAD, grad_bf16, weight_bf16, offsets)
+    return _run_grad_input(grad_bf16, weight_bf16, offsets, grad_bf16.new_empty((t, k)), t, k, n,
+                           experts)
 
 
-def _check_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
-                       out: torch.Tensor) -> None:
-    what = "grouped GEMM gradient"
-    if grad.ndim != 2 or x.ndim != 2 or out.ndim != 3:
-        raise ValueError("grad and x must be 2-D and the output 3-D")
+def _check_grad_weight(grad: torch.Tensor, x: torch.Tensor,
+                       offsets: torch.Tensor) -> tuple[int, int, int, int]:
+    if grad.ndim != 2 or x.ndim != 2:
+        raise ValueError("grad and x must be 2-D")
+    if offsets.ndim != 1 or offsets.shape[0] == 0:
+        raise ValueError("offsets must be 1-D with one entry more than there are experts")
     t, n = grad.shape
-    k = x.shape[1]
-    if x.shape[0] != t:
+    rows, k = x.shape
+    if rows != t:
         raise ValueError("grad and x must have the same number of rows")
-    experts = out.shape[0]
-    if out.shape != (experts, n, k):
-        raise ValueError(f"output shape must be {(experts, n, k)}")
-    _check_offsets(what, offsets, experts)
-    _check_bf16(what, grad, x, out)
-    _check_sizes(what, t, k, n)
+    experts = offsets.shape[0] - 1
+    _check_offsets(_GRAD, offsets, experts)
+    _check_bf16(_GRAD, grad, x)
+    _check_sizes(_GRAD, t, k, n)
+    return t, k, n, experts
 
 
 def _run_grad_weight(grad: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor,
-                     out: torch.Tensor) -> torch.Tensor:
-    experts, n, k = out.shape
+                     out: torch.Tensor, t: int, k: int, n: int, experts: int) -> torch.Tensor:
     if n and k and experts:
         _launch("cuda_operator_gemm_grouped_bf16_grad_weight", grad, _ptr(grad), _ptr(x),
-                _ptr(offsets), _ptr(out), grad.shape[0], k, n, experts)
+                _ptr(offsets), _ptr(out), t, k, n, experts)
     return out
 
 
@@ -200,49 +210,53 @@ def gemm_grouped_bf16_grad_weight_into(grad_bf16: torch.Tensor, x_bf16: torch.Te
     grad [T, N], x [T, K], out [E, N, K], which is written whole: zeros for an
     expert without rows.
     """
-    _check_grad_weight(grad_bf16, x_bf16, offsets, grad_weight_bf16)
-    _check_placement("grouped GEMM gradient", grad_bf16, x_bf16, offsets, grad_weight_bf16)
-    return _run_grad_weight(grad_bf16, x_bf16, offsets, grad_weight_bf16)
+    t, k, n, experts = _check_grad_weight(grad_bf16, x_bf16, offsets)
+    _check_output(_GRAD, grad_weight_bf16, (experts, n, k))
+    _check_placement(_GRAD, grad_bf16, x_bf16, offsets, grad_weight_bf16)
+    return _run_grad_weight(grad_bf16, x_bf16, offsets, grad_weight_bf16, t, k, n, experts)
 
 
 def gemm_grouped_bf16_grad_weight(grad_bf16: torch.Tensor, x_bf16: torch.Tensor,
                                   offsets: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_grouped_bf16_grad_weight_into`."""
-    if grad_bf16.ndim != 2 or x_bf16.ndim != 2:
-        raise ValueError("grad and x must be 2-D and the output 3-D")
-    if offsets.ndim != 1 or offsets.shape[0] == 0:
-        raise ValueError("offsets must be 1-D with one entry more than there are experts")
-    out = torch.empty((offsets.shape[0] - 1, grad_bf16.shape[1], x_bf16.shape[1]),
-                      device=grad_bf16.device, dtype=torch.bfloat16)
-    return gemm_grouped_bf16_grad_weight_into(grad_bf16, x_bf16, offsets, out)
+    t, k, n, experts = _check_grad_weight(grad_bf16, x_bf16, offsets)
+    _check_placement(_GRAD, grad_bf16, x_bf16, offsets)
+    return _run_grad_weight(grad_bf16, x_bf16, offsets, grad_bf16.new_empty((experts, n, k)), t, k,
+                            n, experts)
 
 
 def gemm_grouped_bf16_backward(grad_bf16: torch.Tensor, x_bf16: torch.Tensor,
                                weight_bf16: torch.Tensor,
                                offsets: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Both gradients of :func:`gemm_grouped_bf16`: ``(grad_input, grad_weight)``."""
-    _check_ranks(x_bf16, weight_bf16)
-    grad_input = torch.empty(x_bf16.shape, device=x_bf16.device, dtype=torch.bfloat16)
-    grad_weight = torch.empty(weight_bf16.shape, device=x_bf16.device, dtype=torch.bfloat16)
-    _check_grad_weight(grad_bf16, x_bf16, offsets, grad_weight)
-    _check_grad_input(grad_bf16, weight_bf16, offsets, grad_input)
-    _check_placement("grouped GEMM gradient", grad_bf16, x_bf16, weight_bf16, offsets)
-    return (_run_grad_input(grad_bf16, weight_bf16, offsets, grad_input),
-            _run_grad_weight(grad_bf16, x_bf16, offsets, grad_weight))
+    t, k, n, experts = _check_grad_input(grad_bf16, weight_bf16, offsets)
+    if x_bf16.shape != (t, k):
+        raise ValueError(f"x shape must be {(t, k)}")
+    _check_bf16(_GRAD, x_bf16)
+    _check_placement(_GRAD, grad_bf16, x_bf16, weight_bf16, offsets)
+    return (_run_grad_input(grad_bf16, weight_bf16, offsets, grad_bf16.new_empty((t, k)), t, k, n,
+                            experts),
+            _run_grad_weight(grad_bf16, x_bf16, offsets, grad_bf16.new_empty((experts, n, k)), t,
+                             k, n, experts))
 
 
 # ---------------------------------------------------------------- block-scaled e4m3
 
 
-def _fp8_into(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
-              weight_scale: torch.Tensor, offsets: torch.Tensor,
-              out: torch.Tensor) -> torch.Tensor:
+def _fp8(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: torch.Tensor,
+         weight_scale: torch.Tensor, offsets: torch.Tensor,
+         out: torch.Tensor | None) -> torch.Tensor:
     what = "grouped FP8 GEMM SwiGLU" if swiglu else "grouped FP8 GEMM"
     _check_ranks(x_fp8, weight_fp8)
     experts = weight_fp8.shape[0]
-    t, k, n = _check_fp8_operands(what, x_fp8, x_scale, weight_fp8, weight_scale, out, swiglu)
+    t, k, n = _check_fp8_operands(what, x_fp8, x_scale, weight_fp8, weight_scale, swiglu)
     _check_offsets(what, offsets, experts)
-    _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, offsets, out)
+    if out is None:
+        _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, offsets)
+        out = x_fp8.new_empty((t, n), dtype=torch.bfloat16)
+    else:
+        _check_output(what, out, (t, n))
+        _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, offsets, out)
     if t and n and experts:
         symbol = ("cuda_operator_gemm_grouped_swiglu_fp8_block128" if swiglu
                   else "cuda_operator_gemm_grouped_fp8_block128")
@@ -255,17 +269,14 @@ def gemm_grouped_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Tensor,
                                    weight_fp8: torch.Tensor, weight_scale: torch.Tensor,
                                    offsets: torch.Tensor, out_bf16: torch.Tensor) -> torch.Tensor:
     """:func:`gemm_grouped_bf16_into` of block-scaled e4m3 operands (see ``fp8``)."""
-    return _fp8_into(False, x_fp8, x_scale, weight_fp8, weight_scale, offsets, out_bf16)
+    return _fp8(False, x_fp8, x_scale, weight_fp8, weight_scale, offsets, out_bf16)
 
 
 def gemm_grouped_fp8_block128(x_fp8: torch.Tensor, x_scale: torch.Tensor,
                               weight_fp8: torch.Tensor, weight_scale: torch.Tensor,
                               offsets: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_grouped_fp8_block128_into`."""
-    _check_ranks(x_fp8, weight_fp8)
-    out = torch.empty((x_fp8.shape[0], weight_fp8.shape[1]), device=x_fp8.device,
-                      dtype=torch.bfloat16)
-    return gemm_grouped_fp8_block128_into(x_fp8, x_scale, weight_fp8, weight_scale, offsets, out)
+    return _fp8(False, x_fp8, x_scale, weight_fp8, weight_scale, offsets, None)
 
 
 def gemm_grouped_swiglu_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Tensor,
@@ -273,15 +284,11 @@ def gemm_grouped_swiglu_fp8_block128_into(x_fp8: torch.Tensor, x_scale: torch.Te
                                           weight_scale: torch.Tensor, offsets: torch.Tensor,
                                           out_bf16: torch.Tensor) -> torch.Tensor:
     """:func:`gemm_grouped_swiglu_bf16_into` of block-scaled e4m3 operands; N % 128 == 0."""
-    return _fp8_into(True, x_fp8, x_scale, packed_weight_fp8, weight_scale, offsets, out_bf16)
+    return _fp8(True, x_fp8, x_scale, packed_weight_fp8, weight_scale, offsets, out_bf16)
 
 
 def gemm_grouped_swiglu_fp8_block128(x_fp8: torch.Tensor, x_scale: torch.Tensor,
                                      packed_weight_fp8: torch.Tensor, weight_scale: torch.Tensor,
                                      offsets: torch.Tensor) -> torch.Tensor:
     """Allocating form of :func:`gemm_grouped_swiglu_fp8_block128_into`."""
-    _check_ranks(x_fp8, packed_weight_fp8)
-    out = torch.empty((x_fp8.shape[0], packed_weight_fp8.shape[1] // 2), device=x_fp8.device,
-                      dtype=torch.bfloat16)
-    return gemm_grouped_swiglu_fp8_block128_into(x_fp8, x_scale, packed_weight_fp8, weight_scale,
-                                                 offsets, out)
+    return _fp8(True, x_fp8, x_scale, packed_weight_fp8, weight_scale, offsets, None)
