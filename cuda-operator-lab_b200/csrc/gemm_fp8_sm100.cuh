@@ -40,14 +40,12 @@ constexpr int kFp8RegsReader = 232;
 constexpr int kFp8RegsLaunch = 168;
 static_assert(128 * kFp8RegsControl + 256 * kFp8RegsReader <= 384 * kFp8RegsLaunch, "register shares");
 
-// ROWS = 32: tiles of at most 32 rows, for products whose time is reading w.
-// Only those rows of A are loaded and kept (the MMA's other 96 rows read
-// whatever lies behind them; what they add up is not stored), which leaves the
-// ring to w.  SPLIT: the CTAs of a cluster share a tile's k-blocks and add
-// their sums up in the first one, for a few such tiles.
+// ROWS = 32: tiles of at most 32 rows, of which only those are loaded and kept
+// (as in GroupedCfg).  SPLIT: the CTAs of a cluster share a tile's k-blocks and
+// add their sums up in the first one, for a few such tiles.
 template <int CG, int BN, int ROWS, int SPLIT>
 struct Fp8Cfg {
-  static_assert((ROWS == kBlockM && SPLIT == 1) || (ROWS == 32 && CG == 1), "variants");
+  static_assert((ROWS == kBlockM && SPLIT == 1) || (ROWS == 32 && CG == 1 && SPLIT > 1), "variants");
   static constexpr int kTileRows = ROWS * CG;
   static constexpr int kCols = BN / 2;  // accumulator columns of a reading thread
   static constexpr int kChunk = kCols < 64 ? kCols / 2 : 32;  // columns read at a time
@@ -177,7 +175,6 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
   constexpr int kAccs = Cfg::kAccs;
   constexpr int kGroup = Cfg::kGroup;
   constexpr int kGroups = kKps / kGroup;  // a stage
-  constexpr bool kWrap = ROWS == 32 && SPLIT == 1;  // sums start at first_k
   constexpr uint32_t kIdesc = idesc_e4m3_f32(kBlockM * CG, BN);
   constexpr bool kSplitRegs = fp8_split_regs(BN);
 
@@ -293,12 +290,7 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
               if (j >= nk) break;
               const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
               const uint32_t sb = sa + Cfg::kABytes;
-              int kc = kb + j;
-              if constexpr (kWrap) {
-                kc += t.first_k;
-                if (kc >= kb_end) kc -= kb_end;
-              }
-              kc *= kFp8BlockK;
+              const int kc = (kb + j) * kFp8BlockK;
               if (whole) {
                 grouped_load_2d<CG>(sa, &p.map_a, fb, kc, t.a_row);
               } else {
@@ -433,12 +425,6 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
       uint32_t xs = static_cast<uint32_t>(row_ok ? row : t.begin) * static_cast<uint32_t>(kb_count) + kb_begin;
       const int block = SWIGLU ? t.col / 128 : min((t.col + part_of * kCols) / 128, fp.b_scale_rows - 1);
       uint32_t ws = static_cast<uint32_t>(t.group * fp.b_scale_rows + block) * static_cast<uint32_t>(kb_count) + kb_begin;
-      int left = kb_count;  // k-blocks until the last one's scales
-      if constexpr (kWrap) {
-        left -= t.first_k;
-        xs += t.first_k;
-        ws += t.first_k;
-      }
       const uint32_t wu = SWIGLU ? static_cast<uint32_t>(p.up_offset / 128 * kb_count) : 0u;
       uint64_t sums[kCols / 2];  // two fp32 each
 #pragma unroll
@@ -495,16 +481,8 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
           const float sw = next_x * next_w;
           const float su = next_x * next_u;
           if (kb + 1 < kb_end) {
-            ++xs;
-            ++ws;
-            if constexpr (kWrap) {
-              if (--left == 0) {
-                xs -= kb_count;
-                ws -= kb_count;
-              }
-            }
-            next_x = __ldg(fp.a_scale + xs);
-            next_w = __ldg(fp.b_scale + ws);
+            next_x = __ldg(fp.a_scale + ++xs);
+            next_w = __ldg(fp.b_scale + ++ws);
             if constexpr (SWIGLU) next_u = __ldg(fp.b_scale + ws + wu);
           }
 #pragma unroll

@@ -1,8 +1,7 @@
 // Products grouped by expert (bf16, both gradients, block-scaled e4m3) and the
 // dense block-scaled e4m3 products, which are the same with a single group.
 #include <atomic>
-#include <cstdio>
-#include <cstdlib>
+#include <cmath>
 #include <cstring>
 
 #include "gemm_fp8_sm100.cuh"
@@ -142,6 +141,8 @@ int resident_pairs(Kernel kernel, std::uint32_t smem, int dev) {
   return pairs;
 }
 
+// ---------------------------------------------------------------- choice of tiles
+
 // A tensor-core variant: CTAs of a tile, accumulator columns, rows of a CTA,
 // CTAs that share a tile's sum.
 struct Variant {
@@ -151,15 +152,70 @@ struct Variant {
   int split;
 };
 
-#ifdef EXPERIMENT
-Variant forced(Variant v) {
-  if (const char* f = std::getenv("GROUPED_VARIANT")) {
-    v.cg = f[0] - '0';
-    std::sscanf(f + 1, "%d,%d,%d", &v.bn, &v.rows, &v.split);
-  }
-  return v;
+// What a variant takes, measured under load on a B200 (148 SMs), in us: a
+// k-block of a tile, the same where the tile alone reads its rows of w so that
+// DRAM bounds it, and a tile's share that does not overlap (most of it storing).
+struct VariantCost {
+  Variant v;
+  double block;
+  double block_dram;
+  double tile;
+};
+
+// bf16 (k-blocks of 64).  16384 rows over 8 experts, 4096 x 4096: pairs 398-467
+// us, single CTAs with 256 columns 451-489, with 128 columns 525.  256 rows over
+// 64 experts, gate/up 2048 x 4096: 32-row tiles 144-155 us, 128 columns 154-168,
+// 256 columns 159-164, pairs 222.
+constexpr VariantCost kBf16Costs[] = {
+    {{2, 256, 128, 1}, 0.44, 0.53, 1.8},
+    {{1, 256, 128, 1}, 0.48, 0.72, 1.4},
+    {{1, 128, 128, 1}, 0.285, 0.38, 0.8},
+    {{1, 128, 32, 1}, 0.285, 0.34, 0.8},
+};
+
+// e4m3 (k-blocks of 128).  8192 x 4096 x 4096: pairs 133-150 us, 256 columns
+// 177, 128 columns 195; the decode shape above: 128 columns 85-100 us, 256
+// columns 87-91, pairs 127, 32-row tiles 97 (which therefore serve only sums
+// that a cluster shares).
+constexpr VariantCost kFp8Costs[] = {
+    {{2, 256, 128, 1}, 0.60, 0.66, 1.5},
+    {{1, 256, 128, 1}, 0.79, 0.80, 1.5},
+    {{1, 128, 128, 1}, 0.435, 0.435, 0.8},
+};
+
+// Row tiles of `rows` rows over `groups` groups whose sizes the host does not
+// know: groups without rows have none, the others at least one, and on average
+// half a tile more than their rows fill.
+double expected_row_tiles(std::uint64_t rows, std::uint64_t groups, bool known, int tile_rows) {
+  const double fill = static_cast<double>(rows) / tile_rows;
+  if (known) return static_cast<double>((rows + tile_rows - 1) / tile_rows);
+  const double used = static_cast<double>(rows < groups ? rows : groups);
+  return fill + 0.5 * used > used ? fill + 0.5 * used : used;
 }
-#endif
+
+// The variant whose waves of tiles take least.  `row_tiles(tile_rows)` and
+// `columns` (accumulator columns) span the tiles, `k_blocks` the sum of one.
+template <int COUNT, typename RowTiles>
+Variant choose_variant(const VariantCost (&costs)[COUNT], RowTiles row_tiles, double columns,
+                       double k_blocks, double rows_per_group, int sm_count, bool rows32) {
+  Variant best = costs[0].v;
+  double best_us = -1.0;
+  for (const VariantCost& c : costs) {
+    if (c.v.rows == 32 && !rows32) continue;
+    const int tile_rows = c.v.cg * c.v.rows;
+    // a pair's tile that is not half full is two CTAs' time for one's work
+    if (c.v.cg == 2 && rows_per_group < 128.0) continue;
+    const double tiles = row_tiles(tile_rows) * std::ceil(columns / c.v.bn);
+    const double waves = std::ceil(tiles / (sm_count / c.v.cg));
+    const double block = rows_per_group <= tile_rows ? c.block_dram : c.block;
+    const double us = waves * (k_blocks * block + c.tile);
+    if (best_us < 0.0 || us < best_us) {
+      best = c.v;
+      best_us = us;
+    }
+  }
+  return best;
+}
 
 template <int MODE, bool SWIGLU, int CG, int BN, int ROWS>
 int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int sm_count,
@@ -204,10 +260,19 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   p.up_offset = static_cast<int>(n);
   p.out_vec_ok = col::aligned16(out) && out_cols % 8 == 0;
 
-  Variant v = t >= 256 * experts ? Variant{2, 256, 128, 1} : Variant{1, 128, 128, 1};
-#ifdef EXPERIMENT
-  v = forced(v);
-#endif
+  // Rows a group: of the operand that a tile's rows come from (kGradW: of w, the
+  // same for every group, and the sums have T rows over the groups).
+  const double used = static_cast<double>(t < experts ? t : experts);
+  const double group_rows = static_cast<double>(t) / used;
+  const Variant v = choose_variant(
+      kBf16Costs,
+      [&](int tile_rows) {
+        if (MODE == kGradW) return static_cast<double>(experts * ((n + tile_rows - 1) / tile_rows));
+        return expected_row_tiles(t, experts, false, tile_rows);
+      },
+      static_cast<double>(out_cols * (SWIGLU ? 2 : 1)),
+      MODE == kGradW ? std::ceil(group_rows / 64.0) : static_cast<double>(p.num_k_blocks),
+      MODE == kGradW ? 1e9 : group_rows, info.sm_count, MODE != kGradW);
   p.num_n_blocks = static_cast<int>((out_cols * (SWIGLU ? 2 : 1) + v.bn - 1) / v.bn);
   const std::uint64_t tile_rows = static_cast<std::uint64_t>(v.cg * v.rows);
   const std::uint64_t m_tiles =
@@ -226,10 +291,7 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   const int sms = info.sm_count;
   if (v.cg == 2) return launch_grouped_bf16<MODE, SWIGLU, 2, 256, 128>(p, most_tiles, dev, sms, s);
   if constexpr (MODE != kGradW) {
-    if (v.rows == 32) {
-      if (v.bn == 128) return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 32>(p, most_tiles, dev, sms, s);
-      return launch_grouped_bf16<MODE, SWIGLU, 1, 64, 32>(p, most_tiles, dev, sms, s);
-    }
+    if (v.rows == 32) return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 32>(p, most_tiles, dev, sms, s);
   }
   if (v.bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 1, 256, 128>(p, most_tiles, dev, sms, s);
   return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 128>(p, most_tiles, dev, sms, s);
@@ -296,11 +358,30 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
   fp.b_scale = ws;
   fp.b_scale_rows = static_cast<int>(scale_rows);
 
-  Variant v = t >= 256 * experts ? Variant{2, 256, 128, 1} : Variant{1, 128, 128, 1};
-#ifdef EXPERIMENT
-  v = forced(v);
-  if (k_blocks < static_cast<std::uint64_t>(v.split)) v.split = 1;
-#endif
+  const double used = static_cast<double>(t < experts ? t : experts);
+  Variant v = choose_variant(
+      kFp8Costs,
+      [&](int tile_rows) { return expected_row_tiles(t, experts, offsets == nullptr, tile_rows); },
+      static_cast<double>(w_rows), static_cast<double>(k_blocks), static_cast<double>(t) / used,
+      info.sm_count, false);
+  // A few tiles of few rows: four or two CTAs share each sum while there are
+  // SMs for them, with at least two k-blocks apiece.  One row by 4096 x 4096:
+  // 12.5 us with one CTA a tile, 9.1 with two, 8.1 with four; one row by 1024 x
+  // 4096: 12.2, 8.2, 6.9, and 6.2 with four and 64 columns.
+  const std::uint64_t tiles32 = offsets == nullptr ? (t + 31) / 32 : t / 32 + experts;
+  double best_blocks = 0.0;
+  for (const int bn : {64, 128}) {
+    for (const int split : {2, 4}) {
+      const std::uint64_t ctas = tiles32 * ((w_rows + bn - 1) / bn) * split;
+      if (ctas > static_cast<std::uint64_t>(info.sm_count) || k_blocks < 2u * split) continue;
+      // k-blocks of a CTA, those of 64 columns at 0.7 of the others' time
+      const double blocks = std::ceil(static_cast<double>(k_blocks) / split) * (bn == 64 ? 0.7 : 1.0);
+      if (best_blocks == 0.0 || blocks < best_blocks) {
+        best_blocks = blocks;
+        v = Variant{1, bn, 32, split};
+      }
+    }
+  }
   p.num_n_blocks = static_cast<int>((w_rows + v.bn - 1) / v.bn);
   const std::uint64_t tile_rows = static_cast<std::uint64_t>(v.cg * v.rows);
   const std::uint64_t m_tiles = offsets ? t / tile_rows + experts : (t + tile_rows - 1) / tile_rows;
@@ -317,27 +398,11 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
   if (v.cg == 2) return launch_fp8<SWIGLU, 2, 256, 128, 1>(fp, most_tiles, dev, sms, s);
   if (v.rows == 32) {
     if (v.bn == 128) {
-      switch (v.split) {
-        case 8:
-          return launch_fp8<SWIGLU, 1, 128, 32, 8>(fp, most_tiles, dev, sms, s);
-        case 4:
-          return launch_fp8<SWIGLU, 1, 128, 32, 4>(fp, most_tiles, dev, sms, s);
-        case 2:
-          return launch_fp8<SWIGLU, 1, 128, 32, 2>(fp, most_tiles, dev, sms, s);
-        default:
-          return launch_fp8<SWIGLU, 1, 128, 32, 1>(fp, most_tiles, dev, sms, s);
-      }
+      return v.split == 4 ? launch_fp8<SWIGLU, 1, 128, 32, 4>(fp, most_tiles, dev, sms, s)
+                          : launch_fp8<SWIGLU, 1, 128, 32, 2>(fp, most_tiles, dev, sms, s);
     }
-    switch (v.split) {
-      case 8:
-        return launch_fp8<SWIGLU, 1, 64, 32, 8>(fp, most_tiles, dev, sms, s);
-      case 4:
-        return launch_fp8<SWIGLU, 1, 64, 32, 4>(fp, most_tiles, dev, sms, s);
-      case 2:
-        return launch_fp8<SWIGLU, 1, 64, 32, 2>(fp, most_tiles, dev, sms, s);
-      default:
-        return launch_fp8<SWIGLU, 1, 64, 32, 1>(fp, most_tiles, dev, sms, s);
-    }
+    return v.split == 4 ? launch_fp8<SWIGLU, 1, 64, 32, 4>(fp, most_tiles, dev, sms, s)
+                        : launch_fp8<SWIGLU, 1, 64, 32, 2>(fp, most_tiles, dev, sms, s);
   }
   if (v.bn == 256) return launch_fp8<SWIGLU, 1, 256, 128, 1>(fp, most_tiles, dev, sms, s);
   return launch_fp8<SWIGLU, 1, 128, 128, 1>(fp, most_tiles, dev, sms, s);

@@ -65,7 +65,7 @@ constexpr int b_box_rows(bool swiglu, int cg, int bn) { return swiglu || cg == 2
 // ring to w.
 template <int CG, int BN, int ROWS>
 struct GroupedCfg {
-  static_assert(BN == 64 || BN == 128 || BN == 256, "tile width");
+  static_assert(BN == 128 || BN == 256, "tile width");
   static_assert(CG == 1 || CG == 2, "CTAs of a tile");
   static_assert(ROWS == kBlockM || (ROWS == 32 && CG == 1), "rows of a tile");
   static constexpr int kTileRows = ROWS * CG;
