@@ -57,7 +57,7 @@ struct Fp8Cfg {
   static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
   // one warp's sums of 32 rows, from each other CTA, for two warps
   static constexpr uint32_t kSumBytes = 32 * kCols * 4;
-  static constexpr uint32_t kExtraBytes = 512 + kGroupedTableBytes + (SPLIT - 1) * 2 * kSumBytes;
+  static constexpr uint32_t kExtraBytes = 512 + kGroupTableBytes + (SPLIT - 1) * 2 * kSumBytes;
   static constexpr int kStagesFit =
       static_cast<int>((kSmemLimit - 1024 - kExtraBytes) / kStageBytes);
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
@@ -194,8 +194,8 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
   uint64_t* sums_bar = drain_bar + 1;  // the other CTAs' sums for each of two warps
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sums_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  int* prefix = reinterpret_cast<int*>(smem + kStages * Cfg::kStageBytes + 512);
-  uint8_t* other_sums = smem + kStages * Cfg::kStageBytes + 512 + kGroupedTableBytes;
+  const GroupTables tables = group_tables(smem + kStages * Cfg::kStageBytes + 512);
+  uint8_t* other_sums = smem + kStages * Cfg::kStageBytes + 512 + kGroupTableBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -228,7 +228,7 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
   }
   grid_dependency_wait();
   if (warp == 3) {
-    fill_tile_prefix(prefix, p.offsets, p.groups, p.rows, Cfg::kTileRows, lane);
+    fill_group_tables(tables, p.offsets, p.groups, p.rows, Cfg::kTileRows, lane);
   }
   tc_fence_before();
   if constexpr (CG * SPLIT > 1) {
@@ -242,7 +242,8 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
     atomicOr(p.status, code);
     *abort_flag = 1;
   };
-  const int num_tiles = prefix[p.groups] * p.num_n_blocks;
+  int num_tiles = tables.prefix[p.groups] * p.num_n_blocks;
+  if constexpr (SPLIT > 1) num_tiles = min(num_tiles, workers);  // one tile a cluster
 
   if (warp < 4) {
     if constexpr (kSplitRegs) regs_release<kFp8RegsControl>();
@@ -263,7 +264,7 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
       int filled = 0;
       bool ok = true;
       for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-        const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+        const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
         // Single CTAs load A 32 rows at a time where the group ends early.
         const int rows = min(ROWS, (t.end - t.a_row + 31) & ~31);
         const bool whole = CG == 2 || rows == kBlockM;
@@ -414,7 +415,7 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
     uint32_t slot_phase = 0;  // bit s: parity of slot s's next completion
     bool ok = true;
     for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-      const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+      const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
       const int row = t.a_row + q * 32 + lane;
       const bool row_ok = row < t.end;
       // rows of this warp

@@ -62,8 +62,13 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(const GroupedSimtPara
   // gridDim.y-th.
   int next = blockIdx.y;
   int tiles_before = 0;
+  struct {
+    int begin;
+    int end;
+  } range = {0, p.offsets == nullptr ? 0 : min(max(p.offsets[0], 0), p.rows)};
   for (int g = 0; g < p.groups; ++g) {
-    const RowRange range = group_rows(p.offsets, g, p.rows);
+    range.begin = range.end;
+    range.end = p.offsets == nullptr ? p.rows : max(range.begin, min(max(p.offsets[g + 1], 0), p.rows));
     const int out_rows = MODE == kGradW ? p.n : range.end - range.begin;
     const int depth = MODE == kForward ? p.k : MODE == kGradX ? p.n : range.end - range.begin;
     const int tiles = (out_rows + kTile - 1) / kTile;

@@ -53,9 +53,6 @@ struct __align__(64) GroupedParams {
   int out_vec_ok;    // 16-byte stores allowed
 };
 
-constexpr uint32_t kGroupedTableBytes = 4352;  // prefix table of kMaxGroups + 1 ints
-static_assert(kGroupedTableBytes >= (kMaxGroups + 1) * 4, "table size");
-
 // B is loaded in two boxes where gate and up rows or two CTAs share it.
 constexpr int b_box_rows(bool swiglu, int cg, int bn) { return swiglu || cg == 2 ? bn / 2 : bn; }
 
@@ -74,7 +71,7 @@ struct GroupedCfg {
   static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
   static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : 2;  // k-blocks a stage
   static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
-  static constexpr uint32_t kExtraBytes = 256 + kGroupedTableBytes;
+  static constexpr uint32_t kExtraBytes = 256 + kGroupTableBytes;
   static constexpr int kStagesFit =
       static_cast<int>((kSmemLimit - 1024 - kExtraBytes) / kStageBytes);
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
@@ -204,7 +201,7 @@ __device__ __forceinline__ int few_rows_first_k(int group, int n_block, int num_
 }
 
 template <int MODE, bool SWIGLU, int CG, int BN, int ROWS>
-__device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, const int* prefix,
+__device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, const GroupTables& tables,
                                                     int tile, int rank) {
   constexpr int kTileRows = ROWS * CG;
   GroupedTile t;
@@ -218,15 +215,14 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
     c.m = local % m_blocks;
     c.n = local / m_blocks;
   } else {
-    c = tile_of(tile, prefix, p.groups, p.num_n_blocks);
+    c = tile_of(tile, tables.prefix, p.groups, p.num_n_blocks);
   }
-  const RowRange r = group_rows(p.offsets, c.group, p.rows);
   t.group = c.group;
-  t.begin = r.begin;
-  t.end = r.end;
-  t.a_row = (MODE == kGradW ? 0 : r.begin) + c.m * kTileRows + rank * ROWS;
+  t.begin = tables.starts[c.group];
+  t.end = tables.starts[c.group + 1];
+  t.a_row = (MODE == kGradW ? 0 : t.begin) + c.m * kTileRows + rank * ROWS;
   t.col = c.n * (SWIGLU ? BN / 2 : BN);
-  t.k_blocks = MODE == kGradW ? (r.end - r.begin + kBlockK - 1) / kBlockK : p.num_k_blocks;
+  t.k_blocks = MODE == kGradW ? (t.end - t.begin + kBlockK - 1) / kBlockK : p.num_k_blocks;
   t.first_k = ROWS == 32 ? few_rows_first_k(c.group, c.n, p.num_n_blocks, p.num_k_blocks) : 0;
   return t;
 }
@@ -337,7 +333,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tail_bar + kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   static_assert((3 * kStages + 5) * 8 + 8 <= 256, "barrier space");
-  int* prefix = reinterpret_cast<int*>(smem + kStages * Cfg::kStageBytes + 256);
+  const GroupTables tables = group_tables(smem + kStages * Cfg::kStageBytes + 256);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -371,8 +367,8 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   }
   // The offsets may come from the kernel before this one.
   grid_dependency_wait();
-  if (MODE != kGradW && warp == 3) {
-    fill_tile_prefix(prefix, p.offsets, p.groups, p.rows, Cfg::kTileRows, lane);
+  if (warp == 3) {
+    fill_group_tables(tables, p.offsets, p.groups, p.rows, Cfg::kTileRows, lane);
   }
   tc_fence_before();
   if constexpr (CG == 2) {
@@ -390,7 +386,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   if constexpr (MODE == kGradW) {
     num_tiles = p.groups * ((p.out_rows + Cfg::kTileRows - 1) / Cfg::kTileRows) * p.num_n_blocks;
   } else {
-    num_tiles = prefix[p.groups] * p.num_n_blocks;
+    num_tiles = tables.prefix[p.groups] * p.num_n_blocks;
   }
 
   if (warp == 0) {
@@ -408,7 +404,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     int filled = 0;
     bool ok = true;
     for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
       // Single CTAs load A 32 rows at a time where the group ends early.
       const int rows = min(ROWS, (t.end - t.a_row + 31) & ~31);
       const bool whole = MODE == kGradW || CG == 2 || rows == kBlockM;
@@ -512,7 +508,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       bool ok = true;
       bool issued_any = false;
       for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
         if (MODE == kGradW && t.k_blocks == 0) continue;  // zeros, stored without a sum
         const int acc = local & 1;
         if (!warp_wait(smem_u32(tempty_bar + acc), ((local >> 1) & 1) ^ 1u, abort_flag)) {
@@ -582,7 +578,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       int stage = 0;  // slot of this tile's first stage
       uint32_t tail_phase = 0;  // bit s: parity of tail_bar[s]'s next completion
       for (int tile = worker; tile < num_tiles; tile += workers) {
-        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+        const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
         const int stages = (t.k_blocks + kKps - 1) / kKps;
         const int first = ragged_rows(t);
         if (first != 0) {
@@ -625,7 +621,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     const int half = (warp - 4) >> 2;
     int local = 0;
     for (int tile = worker; tile < num_tiles; tile += workers) {
-      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, prefix, tile, rank);
+      const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
       const int row0 = t.a_row + q * 32;
       // rows of this warp to store; none: they all lie behind the group's last
       const int valid = ROWS == 32 && q != 0

@@ -3,8 +3,9 @@
 // `offsets` (int32 [groups + 1], device memory) sorts the rows of a [rows, *]
 // operand into consecutive groups: group g owns rows [offsets[g],
 // offsets[g + 1]).  The host never reads it (the calls stay capturable), so
-// kernels clamp what they read: whatever the array holds, every row index
-// stays inside [0, rows].
+// kernels take each offset as the largest up to it, clamped to [0, rows]:
+// whatever the array holds, every row index is in range, no row has two groups
+// and the number of tiles keeps its bound.
 #pragma once
 
 #include "common.cuh"
@@ -13,41 +14,60 @@ namespace col {
 
 constexpr int kMaxGroups = 1024;
 
-struct RowRange {
-  int begin;
-  int end;
+// Shared-memory tables of a CTA: first row of each group (starts[groups] ends the
+// last), and the row tiles of the groups before each.
+struct GroupTables {
+  int* starts;
+  int* prefix;
 };
+constexpr unsigned kGroupTableBytes = 2 * 4352;  // kMaxGroups + 1 ints each
+static_assert(kGroupTableBytes / 2 >= (kMaxGroups + 1) * 4, "table size");
 
-// Rows of group g; all of [0, rows) where there is no offsets array.
-__device__ __forceinline__ RowRange group_rows(const int* offsets, int g, int rows) {
-  if (offsets == nullptr) return {0, rows};
-  const int begin = min(max(offsets[g], 0), rows);
-  const int end = min(max(offsets[g + 1], begin), rows);
-  return {begin, end};
+__device__ __forceinline__ GroupTables group_tables(void* smem) {
+  return {static_cast<int*>(smem), static_cast<int*>(smem) + kGroupTableBytes / 8};
 }
 
-// Row tiles of the groups before each group: prefix[g + 1] - prefix[g] =
-// ceil(rows of g / tile_rows).  Written by one warp to shared memory
-// (prefix[0 .. groups]); the CTA synchronises before reading it.
-__device__ __forceinline__ void fill_tile_prefix(int* prefix, const int* offsets, int groups,
-                                                 int rows, int tile_rows, int lane) {
+// Fills the tables from one warp; the CTA synchronises before reading them.
+// Without offsets all rows are one group.
+__device__ __forceinline__ void fill_group_tables(const GroupTables& t, const int* offsets,
+                                                  int groups, int rows, int tile_rows, int lane) {
+  if (offsets == nullptr) {
+    if (lane == 0) {
+      t.starts[0] = 0;
+      t.starts[1] = rows;
+      t.prefix[0] = 0;
+      t.prefix[1] = (rows + tile_rows - 1) / tile_rows;
+    }
+    return;
+  }
+  int highest = 0;  // of the offsets so far
+  for (int g0 = 0; g0 <= groups; g0 += 32) {
+    const int g = g0 + lane;
+    int start = g <= groups ? min(max(offsets[g], 0), rows) : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, start, o);
+      if (lane >= o) start = max(start, v);
+    }
+    start = max(start, highest);
+    if (g <= groups) t.starts[g] = start;
+    highest = __shfl_sync(0xffffffffu, start, 31);
+  }
+  __syncwarp();
   int before = 0;
   for (int g0 = 0; g0 < groups; g0 += 32) {
     const int g = g0 + lane;
     int tiles = 0;
-    if (g < groups) {
-      const RowRange r = group_rows(offsets, g, rows);
-      tiles = (r.end - r.begin + tile_rows - 1) / tile_rows;
-    }
+    if (g < groups) tiles = (t.starts[g + 1] - t.starts[g] + tile_rows - 1) / tile_rows;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, tiles, o);
       if (lane >= o) tiles += v;
     }
-    if (g < groups) prefix[g + 1] = before + tiles;
+    if (g < groups) t.prefix[g + 1] = before + tiles;
     before += __shfl_sync(0xffffffffu, tiles, 31);
   }
-  if (lane == 0) prefix[0] = 0;
+  if (lane == 0) t.prefix[0] = 0;
 }
 
 struct TileCoords {

@@ -7,8 +7,9 @@ the GPU and can be captured in a CUDA graph and replayed with other offsets.
 An expert may have no rows.  Rows of no expert (before ``offsets[0]``, from
 ``offsets[E]`` on, e.g. a batch padded to a fixed T) are neither used nor
 written: the ``_into`` forms leave them as they were, the allocating forms
-return them undefined.  Offsets outside [0, T] are clamped into it, so a wrong
-array gives wrong rows but no access out of range.
+return them undefined.  An offset outside [0, T] is clamped into it and one
+below an earlier offset counts as that one, so a wrong array gives wrong rows
+but no access out of range.
 
 Weights are [E, N, K]; the SwiGLU forms take [E, 2N, K] with the N gate rows
 first, as the dense packed GEMM+SwiGLU does.  Sums are fp32 and outputs bf16.

@@ -313,8 +313,8 @@ int cuda_operator_gemm_swiglu_fp8_block128(const void* input_fp8, const float* i
  * not decreasing) gives expert e the rows offsets[e] .. offsets[e + 1] of the
  * t rows of x; weight [experts, n, k] (swiglu: [experts, 2n, k]).  Rows of no
  * expert (before offsets[0], from offsets[experts] on) are neither used nor
- * written.  Offsets outside [0, t] are clamped, so no call reads or writes out
- * of range.  At most 1024 experts; t == 0, n == 0 or experts == 0 succeeds
+ * written.  An offset counts as the largest up to it, clamped to [0, t], so no
+ * call reads or writes out of range.  At most 1024 experts; t == 0, n == 0 or experts == 0 succeeds
  * first, the other rules are those of the dense forms. */
 int cuda_operator_gemm_grouped_bf16(const void* input_bf16, const void* weight_bf16, const int32_t* offsets, void* output_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
 int cuda_operator_gemm_grouped_swiglu_bf16(const void* input_bf16, const void* packed_weight_bf16, const int32_t* offsets, void* output_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);

@@ -113,7 +113,10 @@ def dequantized(xq, xs, wq, ws):
 # one token to several tiles; k of one block, partial blocks, many blocks; odd n
 PRODUCTS = [(1, 128, 128), (1, 4096, 4096), (2, 16, 16), (7, 129, 144), (16, 1000, 1040),
             (17, 264, 4112), (64, 512, 272), (127, 255, 400), (128, 256, 512), (129, 257, 528),
-            (300, 1001, 2064), (256, 320, 1024), (513, 384, 640), (1025, 640, 896)]
+            (300, 1001, 2064), (256, 320, 1024), (513, 384, 640), (1025, 640, 896),
+            # sums shared by the CTAs of a cluster, 64 and 128 columns a tile
+            (3, 200, 14336), (32, 4096, 1040), (33, 600, 2064), (40, 2900, 1040), (96, 1000, 784),
+            (5, 4100, 4096)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -126,7 +129,8 @@ def test_gemm(m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(1, 128, 128), (1, 2048, 4096), (5, 256, 400), (130, 384, 1040),
-                                   (257, 128, 2064), (600, 640, 528)])
+                                   (257, 128, 2064), (600, 640, 528), (2, 256, 8208),
+                                   (31, 1024, 1040), (70, 512, 2064)])
 def test_gemm_swiglu(m, n, k):
     args = operands(m, n, k, seeded(m + n + k), swiglu=True)
     y = fp8.gemm_swiglu_fp8_block128(*args)

@@ -6,11 +6,14 @@ are exact in every type on the way, so most checks there are of equality.
 
 from __future__ import annotations
 
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import expert_math as em
-from conftest import seeded
+from conftest import PACKAGE_DIR, seeded
 from cuda_operator_lab import bindings as b
 from cuda_operator_lab import fp8, grouped
 
@@ -66,6 +69,79 @@ def test_forward_swiglu(name, n, k):
     assert b.gemm_status() == 0
     for e, (lo, hi) in enumerate(groups(lengths)):
         em.assert_within(y[lo:hi].cpu(), *em.product(x[lo:hi].double(), w[e].double(), True))
+
+
+# One size at least for each tile shape that the library chooses from: few rows
+# an expert, half-filled tiles, several whole ones.
+TILES = [([300, 513, 0, 129], 136, 144), ([300, 513, 0, 129], 2000, 144),
+         ([300, 513, 0, 129], 136, 2064), ([700, 0, 650], 2000, 2064), ([700, 0, 650], 1000, 2064),
+         ([100] * 16, 136, 144), ([90, 70, 0, 110, 128, 60], 1000, 528),
+         ([20] * 10, 264, 2064), ([5, 0, 40, 3], 264, 2064)]
+
+
+def pairs_of(lengths):
+    return [(e, slice(lo, hi)) for e, (lo, hi) in enumerate(groups(lengths))]
+
+
+@pytest.mark.parametrize("lengths,n,k", TILES)
+def test_tile_shapes_bf16(lengths, n, k):
+    g = seeded(n + k + len(lengths))
+    t, off = sum(lengths), em.offsets_of(lengths).to(DEV)
+    x = torch.randn(t, k, generator=g).bfloat16().to(DEV)
+    grad = torch.randn(t, n, generator=g).bfloat16().to(DEV)
+    w = (torch.randn(len(lengths), 2 * n, k, generator=g) * k ** -0.5).bfloat16().to(DEV)
+    one = w[:, :n].contiguous()
+    y, h = grouped.gemm_grouped_bf16(x, one, off), grouped.gemm_grouped_swiglu_bf16(x, w, off)
+    dx, dw = grouped.gemm_grouped_bf16_backward(grad, x, one, off)
+    assert b.gemm_status() == 0
+    for e, r in pairs_of(lengths):
+        xr, gr, we = x[r].double(), grad[r].double(), w[e].double()
+        em.assert_within(y[r], *em.product(xr, we[:n], False))
+        em.assert_within(h[r], *em.product(xr, we, True))
+        em.assert_within(dx[r], *em.product(gr, we[:n].mT, False))
+        em.assert_within(dw[e], *em.product(gr.mT, xr.mT, False))
+
+
+def test_tile_shapes_of_long_batches():
+    """Thousands of rows an expert: the widest tiles of all four products."""
+    lengths, n, k = [2001, 1950, 0, 2300], 1032, 2048
+    g = seeded(21)
+    t, off = sum(lengths), em.offsets_of(lengths).to(DEV)
+    x = torch.randn(t, k, generator=g).bfloat16().to(DEV)
+    grad = torch.randn(t, n, generator=g).bfloat16().to(DEV)
+    w = (torch.randn(4, n, k, generator=g) * k ** -0.5).bfloat16().to(DEV)
+    y = grouped.gemm_grouped_bf16(x, w, off)
+    dx, dw = grouped.gemm_grouped_bf16_backward(grad, x, w, off)
+    xq, xs, wq, ws = quantized(x, w)
+    y8 = grouped.gemm_grouped_fp8_block128(xq, xs, wq, ws, off)
+    assert b.gemm_status() == 0
+    xd, wd = xq.double() * em.spread(xs, 1, t, k), wq.double() * em.spread(ws, 128, n, k)
+    for e, r in pairs_of(lengths):
+        xr, gr, we = x[r].double(), grad[r].double(), w[e].double()
+        em.assert_within(y[r], *em.product(xr, we, False))
+        em.assert_within(dx[r], *em.product(gr, we.mT, False))
+        em.assert_within(dw[e], *em.product(gr.mT, xr.mT, False))
+        em.assert_within(y8[r], *em.product(xd[r], wd[e], False))
+
+
+@pytest.mark.parametrize("lengths,n,k", TILES + [([300, 513, 0, 129], 136, 528),
+                                                 ([20] * 10, 136, 2064), ([20] * 10, 264, 528),
+                                                 ([100] * 16, 1000, 144),
+                                                 ([90, 70, 0, 110, 128, 60], 136, 528),
+                                                 ([5, 0, 40, 3], 136, 2064)])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_tile_shapes_fp8(lengths, n, k, swiglu):
+    n = -(-n // 128) * 128 if swiglu else n
+    g = seeded(n + k + len(lengths))
+    x = torch.randn(sum(lengths), k, generator=g) * torch.exp(torch.randn(k, generator=g))
+    w = torch.randn(len(lengths), 2 * n if swiglu else n, k, generator=g) * k ** -0.5
+    xq, xs, wq, ws = quantized(x, w)
+    gemm = grouped.gemm_grouped_swiglu_fp8_block128 if swiglu else grouped.gemm_grouped_fp8_block128
+    y = gemm(xq, xs, wq, ws, em.offsets_of(lengths).to(DEV))
+    assert b.gemm_status() == 0
+    xd, wd = xq.double() * em.spread(xs, 1, *x.shape), wq.double() * em.spread(ws, 128, *w.shape[1:])
+    for e, r in pairs_of(lengths):
+        em.assert_within(y[r], *em.product(xd[r], wd[e], swiglu))
 
 
 @pytest.mark.parametrize("lengths", [[5, 0, 40, 3], [300, 513, 0, 129], [2] * 48])
@@ -236,6 +312,59 @@ def test_wrong_offsets_stay_in_range(wrong):
         assert (whole[:guard] == 7).all() and (whole[-guard:] == 7).all()
 
 
+@pytest.mark.parametrize("wrong", [[-50, 10, 20, 30], [0, 40, 10, 60], [0, 10, 900, 2 ** 31 - 1],
+                                   [7, 3, 50, 20], [500, 600, 700, 800], [-2 ** 31, -7, -3, -1]])
+def test_offsets_count_as_the_largest_up_to_them(wrong):
+    """Offsets that decrease or leave [0, T] act as their clamped running maximum:
+    no row has two experts, rows of none are not written."""
+    t, n, k = 60, 72, 48
+    right = torch.tensor(wrong).clamp(0, t).cummax(0).values.int()
+    g = seeded(35)
+    x, grad = em.small_integers((t, k), g, 1), em.small_integers((t, n), g, 1)
+    w = em.small_integers((3, n, k), g, 1)
+    got, want = [], []
+    for off, results in ((torch.tensor(wrong, dtype=torch.int32), got), (right, want)):
+        off = off.to(DEV)
+        for xs, ws, gs in ((bf(x), bf(w), bf(grad)), (bf(x[:, :-1]), bf(w[:, :-1, :-1]), bf(grad[:, :-1]))):
+            y = torch.full((t, ws.shape[1]), 7.0, device=DEV, dtype=torch.bfloat16)
+            dx = torch.full((t, ws.shape[2]), 7.0, device=DEV, dtype=torch.bfloat16)
+            results.append(grouped.gemm_grouped_bf16_into(xs, ws, off, y))
+            results.append(grouped.gemm_grouped_bf16_grad_input_into(gs, ws, off, dx))
+            results.append(grouped.gemm_grouped_bf16_grad_weight(gs, xs, off))
+    assert b.gemm_status() == 0
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    ends = right.tolist()
+    for e, (lo, hi) in enumerate(zip(ends[:-1], ends[1:])):
+        assert torch.equal(got[0][lo:hi].float().cpu(), x[lo:hi] @ w[e].t())
+    assert (got[0][:ends[0]] == 7).all() and (got[0][ends[-1]:] == 7).all()
+
+
+def test_most_experts():
+    """1024 experts, most with a row or two, some with none."""
+    experts, n, k = grouped.MAX_EXPERTS, 40, 24
+    g = seeded(36)
+    lengths = torch.randint(0, 4, (experts,), generator=g).tolist()
+    t, off = sum(lengths), em.offsets_of(lengths).to(DEV)
+    x, grad = em.small_integers((t, k), g, 1), em.small_integers((t, n), g, 1)
+    w = em.small_integers((experts, n, k), g, 1)
+    owner = torch.repeat_interleave(torch.arange(experts), torch.tensor(lengths))
+    y = grouped.gemm_grouped_bf16(bf(x), bf(w), off)
+    dx, dw = grouped.gemm_grouped_bf16_backward(bf(grad), bf(x), bf(w), off)
+    assert b.gemm_status() == 0
+    assert torch.equal(y.float().cpu(), torch.einsum("tk,tnk->tn", x, w[owner]))
+    assert torch.equal(dx.float().cpu(), torch.einsum("tn,tnk->tk", grad, w[owner]))
+    want = torch.zeros(experts, n, k).index_add_(0, owner, grad[:, :, None] * x[:, None, :])
+    assert torch.equal(dw.float().cpu(), want)
+    x8, w8 = torch.randn(t, 144, generator=g), torch.randn(experts, n, 144, generator=g)
+    xq, xs, wq, ws = quantized(x8, w8)
+    y8 = grouped.gemm_grouped_fp8_block128(xq, xs, wq, ws, off)
+    xd, wd = xq.double() * em.spread(xs, 1, t, 144), wq.double() * em.spread(ws, 128, n, 144)
+    own = owner.to(DEV)
+    h = torch.einsum("tk,tnk->tn", xd, wd[own])
+    err = (144 + 8) * 2.0 ** -23 * torch.einsum("tk,tnk->tn", xd.abs(), wd[own].abs())
+    em.assert_within(y8, h, err + em.HALF_STEP_BF16 * (h.abs() + err))
+
+
 def test_no_rows_at_all():
     w = torch.randn(2, 64, 32, device=DEV).bfloat16()
     off = torch.zeros(3, dtype=torch.int32, device=DEV)
@@ -355,6 +484,34 @@ def test_captured_layer_replays_with_other_offsets():
             assert torch.equal(got, w)
     assert b.gemm_status() == 0
     del graph
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing that the library sets up on its first call breaks a capture."""
+    code = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from cuda_operator_lab import bindings, fp8, grouped
+x = torch.ones(40, 256, device="cuda", dtype=torch.bfloat16)
+w = torch.ones(2, 256, 256, device="cuda", dtype=torch.bfloat16)
+off = torch.tensor([0, 30, 40], dtype=torch.int32, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = grouped.gemm_grouped_bf16(x, w, off)
+    dx, dw = grouped.gemm_grouped_bf16_backward(y, x, w, off)
+    y8 = grouped.gemm_grouped_fp8_block128(
+        *fp8.quantize_fp8_block128(x), *fp8.quantize_fp8_block128_weight(w), off)
+graph.replay()
+torch.cuda.synchronize()
+assert (y == 256).all() and (y8 == 256).all() and (dx == 65536).all()
+assert (dw[0] == 7680).all() and (dw[1] == 2560).all()
+assert bindings.gemm_status() == 0
+print("captured")
+"""
+    done = subprocess.run([sys.executable, "-c", code, str(PACKAGE_DIR)], capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
 
 
 def test_two_streams_at_once():
