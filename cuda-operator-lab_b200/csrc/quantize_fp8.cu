@@ -2,8 +2,17 @@
 // or 128 x 128 tile (weights).
 //
 //   a = max(max |x| over the block, 2^-100)
-//   scale = a / 448        inverse = 448 / a      (fp32, IEEE division)
-//   q = e4m3(x * inverse), to nearest even, saturating
+//   scale = a / 448                    (fp32, IEEE division)
+//   q = e4m3(x * 448 / a), to nearest even of the exact quotient
+//
+// v = x * (448 / a) in fp32 is up to 2 units in its last place off the quotient
+// and rounds wrongly where a tie of two e4m3 values lies between (with bf16
+// inputs quotients that are ties are common: 3 in 10^4 values of a normal sample
+// came out one step off).  One Newton step on the residual v a - 448 x gives the
+// quotient correctly rounded: then v is on the quotient's side of every tie, or
+// is a tie itself.  With bf16 inputs the quotient then is that tie (two 8-bit
+// significands: any other quotient is at least 2^-13 away).  With fp32 inputs it
+// may lie beside it, and the sign of t a - 448 x for the tie t decides.
 //
 // 448 is e4m3's largest value, so a block always uses the whole range.  The
 // floor keeps the inverse finite: an all-zero block gives q = 0 with scale
@@ -12,8 +21,7 @@
 // 448 / inf), so a product over either block is NaN, never a plausible number.
 // The maximum is taken over the bit patterns of |x| as integers, which order
 // like the values and put NaN above infinity, where fmaxf would drop it.
-// One division a block and one multiplication an element: the kernels are
-// bound by memory, one read of x and one write of q.
+// The kernels are bound by memory, one read of x and one write of q.
 #include <cuda_fp8.h>
 
 #include "common.cuh"
@@ -82,39 +90,109 @@ __device__ __forceinline__ float block_amax(unsigned m) {
   return __uint_as_float(max(m, kAmaxFloorBits));
 }
 
+// What the values of a block are multiplied by and corrected with.  The residual
+// is taken of x * 448 and a both times 2^-10, against overflow.  A block with an
+// infinity is not corrected: x * 0 is its result.
+struct BlockScale {
+  float inverse;   // 448 / a
+  float a10;       // a 2^-10
+  float step;      // 1 / a10
+  __device__ __forceinline__ explicit BlockScale(float amax) {
+    inverse = __fdiv_rn(kE4m3Max, amax);
+    const bool finite = __float_as_uint(amax) < 0x7f800000u;
+    a10 = finite ? amax * 0x1p-10f : 0.0f;
+    step = finite ? inverse * (1024.0f / 448.0f) : 0.0f;
+  }
+};
+constexpr float kE4m3Max10 = 0.4375f;  // 448 2^-10
+
+// The correctly rounded quotient v, or where it is a tie its neighbour on the
+// side of the exact one.
+__device__ __forceinline__ float settle_tie(float x, float v, float a10) {
+  const unsigned b = __float_as_uint(v) & 0x7fffffffu;
+  const float t = __uint_as_float(b);
+  // normal values: half of the 20 bits that e4m3 drops; below, where the ties are
+  // multiples of 2^-10, as e4m3's values are, for which nothing changes
+  const bool tie = b >= 0x3c800000u ? (b & 0xfffffu) == 0x80000u
+                                    : __fsub_rn(__fadd_rn(t, 12288.0f), 12288.0f) == t;
+  if (!tie) return v;
+  // every step is exact: t has at most 5 significant bits
+  const float hi = __fmul_rn(fabsf(x), kE4m3Max10);
+  const float lo = __fmaf_rn(fabsf(x), kE4m3Max10, -hi);
+  const float d = __fsub_rn(__fmaf_rn(t, a10, -hi), lo);
+  unsigned r = b;
+  if (d < 0.0f) r += 1u;
+  if (d > 0.0f) r -= 1u;
+  return __uint_as_float(r | (__float_as_uint(v) & 0x80000000u));
+}
+
+// x * 448 / a, on the right side of every tie.
+template <typename T>
+__device__ __forceinline__ float quotient(float x, const BlockScale& s) {
+  const float v = x * s.inverse;
+  const float hi = __fmul_rn(x, kE4m3Max10);  // exact for bf16
+  float d = __fmaf_rn(v, s.a10, -hi);
+  if constexpr (sizeof(T) == 4) d = __fsub_rn(d, __fmaf_rn(x, kE4m3Max10, -hi));
+  return __fmaf_rn(-d, s.step, v);
+}
+
 template <typename T, bool VEC>
 __device__ __forceinline__ void store8(__nv_fp8_storage_t* q, int left, const Raw8<T>& r,
-                                       float inverse) {
+                                       const BlockScale& s) {
   if (left <= 0) return;
   unsigned w[4];
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 f;
-    if constexpr (sizeof(T) == 2) {
-      f = make_float2(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
-    } else {
-      f = make_float2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+    for (int i = 0; i < 4; ++i) {
+      w[i] = __nv_cvt_float2_to_fp8x2(
+          make_float2(quotient<T>(__uint_as_float(r.w[i] << 16), s),
+                      quotient<T>(__uint_as_float(r.w[i] & 0xffff0000u), s)),
+          __NV_SATFINITE, __NV_E4M3);
     }
-    f.x *= inverse;
-    f.y *= inverse;
-    w[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  } else {
+    // Bounds of the quotient, 2^-22 to either side: where both round alike, so
+    // does the quotient.  Else (one value in 10^6) it is computed.
+    const float below = s.inverse * (1.0f - 0x1p-22f);
+    const float above = s.inverse * (1.0f + 0x1p-22f);
+    unsigned differ = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x0 = __uint_as_float(r.w[2 * i]);
+      const float x1 = __uint_as_float(r.w[2 * i + 1]);
+      w[i] = __nv_cvt_float2_to_fp8x2(make_float2(x0 * below, x1 * below), __NV_SATFINITE, __NV_E4M3);
+      differ |= w[i] ^ __nv_cvt_float2_to_fp8x2(make_float2(x0 * above, x1 * above),
+                                                __NV_SATFINITE, __NV_E4M3);
+    }
+    if (differ != 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float v[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float x = __uint_as_float(r.w[2 * i + j]);
+          v[j] = settle_tie(x, quotient<T>(x, s), s.a10);
+        }
+        w[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3);
+      }
+    }
   }
-  const uint2 v = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+  const uint2 bytes = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
   if constexpr (VEC) {
-    *reinterpret_cast<uint2*>(q) = v;
+    *reinterpret_cast<uint2*>(q) = bytes;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (i < left) q[i] = static_cast<__nv_fp8_storage_t>(((i < 4 ? v.x : v.y) >> (8 * (i & 3))) & 0xffu);
+      if (i < left) q[i] = static_cast<__nv_fp8_storage_t>(((i < 4 ? bytes.x : bytes.y) >> (8 * (i & 3))) & 0xffu);
     }
   }
 }
 
 // Rows: block b of all rows * kb blocks belongs to 8 lanes of two 16-byte loads
 // (bf16) each, which read 128 contiguous bytes at a time.  bf16 [16384, 4096]
-// takes 29.9 us, 6.7 TB/s; 16 lanes with one load 39.8 (twice the divisions and
-// shuffles a byte), several blocks a thread 30.2 and more (fewer threads), values
-// kept as floats instead of as loaded 42.4 (registers).  fp32: 47.9 us, 7.0 TB/s.
+// takes 33.0 us, 6.1 TB/s, fp32 48.2 us, 7.0 TB/s.  Before the correction to exact
+// quotients bf16 took 29.9 us; 16 lanes with one load 39.8 (twice the divisions
+// and shuffles a byte), several blocks a thread 30.2 and more (fewer threads),
+// values kept as floats instead of as loaded 42.4 (registers).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     quantize_rows_kernel(const T* __restrict__ x, __nv_fp8_storage_t* __restrict__ q,
@@ -150,17 +228,17 @@ __global__ void __launch_bounds__(kThreads)
     m = sizeof(T) == 2 ? __vmaxu2(m, other) : max(m, other);
   }
   const float amax = block_amax<T>(m);
-  const float inverse = __fdiv_rn(kE4m3Max, amax);
+  const BlockScale block(amax);
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    store8<T, VEC>(q + at + i * kRowLanes * 8, left - i * kRowLanes * 8, raw[i], inverse);
+    store8<T, VEC>(q + at + i * kRowLanes * 8, left - i * kRowLanes * 8, raw[i], block);
   }
   if (lane == 0 && b < blocks) scale[b] = __fdiv_rn(amax, kE4m3Max);
 }
 
 // Weights: one CTA a 128 x 128 tile, held in registers between the maximum
-// and the rounding (8 rows of 8 columns a thread).  fp32 [6, 1900, 2064]: 21.6
-// us with the call, 5.4 TB/s.
+// and the rounding (8 rows of 8 columns a thread).  fp32 [6, 1900, 2064]: 22.6
+// us with the call, 5.2 TB/s.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
     quantize_tiles_kernel(const T* __restrict__ w, __nv_fp8_storage_t* __restrict__ q,
@@ -192,12 +270,12 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
   for (int i = 0; i < kThreads / 32; ++i) m = max(m, warp_max[i]);
   const float amax = __uint_as_float(max(m, kAmaxFloorBits));
-  const float inverse = __fdiv_rn(kE4m3Max, amax);
+  const BlockScale block(amax);
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
     const unsigned row = row0 + i * (kThreads / kLanes);
     const int left = row < n ? static_cast<int>(k) - static_cast<int>(col) : 0;
-    store8<T, VEC>(q + (base + row) * k + col, left, raw[i], inverse);
+    store8<T, VEC>(q + (base + row) * k + col, left, raw[i], block);
   }
   if (threadIdx.x == 0) scale[blockIdx.x] = __fdiv_rn(amax, kE4m3Max);
 }

@@ -4,8 +4,9 @@ A matrix is held as ``torch.float8_e4m3fn`` values beside fp32 scales: one for
 each 128 columns of a row (activations, ``[M, ceil(K/128)]``) or for each
 128 x 128 tile (weights, ``[N/128, K/128]`` rounded up, with the experts in
 front where there are several).  For a block with largest magnitude ``a`` (at
-least 2**-100) the scale is ``a / 448`` and the values are ``x * (448 / a)``
-rounded to nearest even, so ``q.float() * scale`` stands for ``x``.  A NaN or
+least 2**-100) the scale is ``a / 448`` and the values are ``x * 448 / a`` rounded
+to nearest even (of the exact quotient), so ``q.float() * scale`` stands for
+``x``.  A NaN or
 an infinity in a block makes every product over that block NaN.
 
 As in ``bindings``: contiguous CUDA tensors, the current stream of the

@@ -294,7 +294,7 @@ int cuda_operator_lab_reduction_noalloc(const float* input, float* output, uint6
  * (activations, scale [m, ceil(k/128)]) or each 128 x 128 tile (weights, scale
  * [experts, ceil(n/128), ceil(k/128)]):
  *   a = max(max |x| over the block, 2^-100), scale = a / 448,
- *   q = e4m3(x * (448 / a)), to nearest even.
+ *   q = e4m3(x * 448 / a), to nearest even of the exact quotient.
  * A block that holds a NaN or an infinity makes every product over it NaN. */
 int cuda_operator_quantize_fp8_block128_f32(const float* input, void* output_fp8, float* scale, uint64_t m, uint64_t k, void* stream);
 int cuda_operator_quantize_fp8_block128_bf16(const void* input_bf16, void* output_fp8, float* scale, uint64_t m, uint64_t k, void* stream);
