@@ -237,10 +237,12 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // Weights: one CTA a 128 x 128 tile, held in registers between the maximum
-// and the rounding (8 rows of 8 columns a thread).  fp32 [6, 1900, 2064]: 22.6
-// us with the call, 5.2 TB/s.
+// and the rounding (8 rows of 8 columns a thread).
+// Three CTAs an SM for bf16: [16, 2048, 4096] 78.2 -> 68.2 us, 5.9 TB/s (four
+// spill: 84.6); two for fp32, whose values take twice the registers: 100.5 us, 6.7
+// TB/s (three: 137.6).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
     quantize_tiles_kernel(const T* __restrict__ w, __nv_fp8_storage_t* __restrict__ q,
                           float* __restrict__ scale, unsigned n, unsigned k, unsigned nb,
                           unsigned kb) {
