@@ -21,7 +21,8 @@ from __future__ import annotations
 import torch
 from torch._C import _cuda_getDevice as _current_device
 
-from .bindings import _call, _ptr, _stream
+from . import bindings
+from .bindings import _ptr, _stream
 
 __all__ = [
     "quantize_fp8_block128", "quantize_fp8_block128_into",
@@ -70,11 +71,14 @@ def _check_sizes(what: str, *sizes: int) -> None:
 
 def _launch(symbol: str, on: torch.Tensor, *args) -> None:
     """One library call on the current stream of ``on``'s device."""
+    library = bindings._LIBRARY or bindings._library()
     if on.get_device() == _current_device():
-        _call(symbol, *args, _stream(on))
+        code = library.functions[symbol](*args, _stream(on))
     else:
         with torch.cuda.device(on.device):
-            _call(symbol, *args, _stream(on))
+            code = library.functions[symbol](*args, _stream(on))
+    if code:
+        library.check(code)
 
 
 # ---------------------------------------------------------------- quantisation
@@ -186,9 +190,13 @@ def _check_fp8_operands(what: str, x_fp8: torch.Tensor, x_scale: torch.Tensor,
     m, k = x_fp8.shape
     w_shape = weight_fp8.shape
     w_rows = w_shape[-2]
+    blocks = _blocks(k)
+    if len(w_shape) == 2:
+        scale_shape = (_blocks(w_rows), blocks)
+    else:
+        scale_shape = (w_shape[0], _blocks(w_rows), blocks)
     if (w_shape[-1] == k and k > 0 and not (swiglu and w_rows % (2 * BLOCK))
-            and x_scale.shape == (m, _blocks(k))
-            and weight_scale.shape == (*w_shape[:-2], _blocks(w_rows), _blocks(k))
+            and x_scale.shape == (m, blocks) and weight_scale.shape == scale_shape
             and x_fp8.dtype is _E4M3 and weight_fp8.dtype is _E4M3
             and x_scale.dtype is torch.float32 and weight_scale.dtype is torch.float32
             and m <= _MAX_SIZE and k <= _MAX_SIZE and w_rows <= _MAX_SIZE):
@@ -199,10 +207,10 @@ def _check_fp8_operands(what: str, x_fp8: torch.Tensor, x_scale: torch.Tensor,
         raise ValueError(f"{what} requires k > 0")
     if swiglu and w_rows % (2 * BLOCK):
         raise ValueError(f"{what} needs gate and up rows in whole blocks of {BLOCK}")
-    if x_scale.shape != (m, _blocks(k)):
-        raise ValueError(f"x scale shape must be {(m, _blocks(k))}")
-    if weight_scale.shape != _weight_scale_shape(w_shape):
-        raise ValueError(f"weight scale shape must be {_weight_scale_shape(w_shape)}")
+    if x_scale.shape != (m, blocks):
+        raise ValueError(f"x scale shape must be {(m, blocks)}")
+    if weight_scale.shape != scale_shape:
+        raise ValueError(f"weight scale shape must be {scale_shape}")
     if x_fp8.dtype != _E4M3 or weight_fp8.dtype != _E4M3:
         raise TypeError(f"{what} expects float8_e4m3fn x and weight")
     if x_scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:

@@ -25,8 +25,8 @@ from __future__ import annotations
 import torch
 
 from .bindings import _ptr
-from .fp8 import (_check_fp8_operands, _check_output, _check_placement, _check_sizes, _launch,
-                  _MAX_SIZE)
+from .fp8 import (_MAX_SIZE, _check_fp8_operands, _check_output, _check_placement, _check_sizes,
+                  _launch)
 
 __all__ = [
     "gemm_grouped_bf16", "gemm_grouped_bf16_into",
