@@ -164,7 +164,6 @@ __device__ __forceinline__ float2 unpack2(uint64_t v) {
   return f;
 }
 
-
 template <bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
 __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads, 1)
     fp8_kernel(const __grid_constant__ Fp8Params fp) {
@@ -471,9 +470,11 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
           }
           return t_lane + (acc * kGroup + in_group) * BN + col;
         };
-        float next_x = __ldg(fp.a_scale + xs);
-        float next_w = __ldg(fp.b_scale + ws);
-        float next_u = SWIGLU ? __ldg(fp.b_scale + ws + wu) : 0.0f;
+        // Plain loads: the kernel that writes the scales may still have been running
+        // when this one started, which non-coherent loads do not allow for.
+        float next_x = fp.a_scale[xs];
+        float next_w = fp.b_scale[ws];
+        float next_u = SWIGLU ? fp.b_scale[ws + wu] : 0.0f;
         uint32_t part[2][kChunk];
         ok = next_group(kb_begin);
         if (ok) tmem_ld_start(chunk_addr(0), part[0]);
@@ -482,9 +483,9 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
           const float sw = next_x * next_w;
           const float su = next_x * next_u;
           if (kb + 1 < kb_end) {
-            next_x = __ldg(fp.a_scale + ++xs);
-            next_w = __ldg(fp.b_scale + ++ws);
-            if constexpr (SWIGLU) next_u = __ldg(fp.b_scale + ws + wu);
+            next_x = fp.a_scale[++xs];
+            next_w = fp.b_scale[++ws];
+            if constexpr (SWIGLU) next_u = fp.b_scale[ws + wu];
           }
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {

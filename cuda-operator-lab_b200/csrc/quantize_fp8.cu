@@ -195,7 +195,7 @@ __device__ __forceinline__ void store8(__nv_fp8_storage_t* q, int left, const Ra
 // values kept as floats instead of as loaded 42.4 (registers).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-    quantize_rows_kernel(const T* __restrict__ x, __nv_fp8_storage_t* __restrict__ q,
+    quantize_rows_kernel(const T* x, __nv_fp8_storage_t* __restrict__ q,
                          float* __restrict__ scale, unsigned long long blocks, unsigned kb,
                          unsigned k) {
   grid_dependency_wait();
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads)
 // TB/s (three: 137.6).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 3 : 2)
-    quantize_tiles_kernel(const T* __restrict__ w, __nv_fp8_storage_t* __restrict__ q,
+    quantize_tiles_kernel(const T* w, __nv_fp8_storage_t* __restrict__ q,
                           float* __restrict__ scale, unsigned n, unsigned k, unsigned nb,
                           unsigned kb) {
   grid_dependency_wait();
