@@ -17,7 +17,6 @@
 #pragma once
 
 #include "gemm_grouped_sm100.cuh"
-#include "gemm_sm100_sk.cuh"
 
 namespace col {
 namespace sm100 {
@@ -133,16 +132,6 @@ __device__ __forceinline__ uint64_t pack2(float x, float y) {
   uint64_t v;
   asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
   return v;
-}
-
-// warp_wait on data that other CTAs of the cluster wrote.
-__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity,
-                                                  volatile int* abort_flag) {
-  for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if ((i & 63u) == 0u && *abort_flag) break;
-  }
-  return false;
 }
 
 // sums += part * scale, two columns an instruction.

@@ -193,6 +193,14 @@ double expected_row_tiles(std::uint64_t rows, std::uint64_t groups, bool known, 
   return fill + 0.5 * used > used ? fill + 0.5 * used : used;
 }
 
+// The most row tiles there can be: each has at least one row, each group at most
+// one that is not full.
+std::uint64_t most_row_tiles(std::uint64_t rows, std::uint64_t groups, bool known, int tile_rows) {
+  if (known) return (rows + tile_rows - 1) / tile_rows;
+  const std::uint64_t tiles = rows / tile_rows + groups;
+  return tiles < rows ? tiles : rows;
+}
+
 // The variant whose waves of tiles take least.  `row_tiles(tile_rows)` and
 // `columns` (accumulator columns) span the tiles, `k_blocks` the sum of one.
 template <int COUNT, typename RowTiles>
@@ -217,11 +225,11 @@ Variant choose_variant(const VariantCost (&costs)[COUNT], RowTiles row_tiles, do
   return best;
 }
 
-template <int MODE, bool SWIGLU, int CG, int BN, int ROWS>
+template <int MODE, bool SWIGLU, int CG, int BN, int ROWS, int SPLIT = 1>
 int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int sm_count,
                         cudaStream_t s) {
-  using Cfg = GroupedCfg<CG, BN, ROWS>;
-  auto kernel = col::sm100::grouped_bf16_kernel<MODE, SWIGLU, CG, BN, ROWS>;
+  using Cfg = GroupedCfg<CG, BN, ROWS, SPLIT>;
+  auto kernel = col::sm100::grouped_bf16_kernel<MODE, SWIGLU, CG, BN, ROWS, SPLIT>;
   static std::atomic<std::uint64_t> done{0};
   if (int rc = allow_smem(kernel, Cfg::kSmemBytes, dev, done)) return rc;
   int workers = sm_count;
@@ -229,8 +237,11 @@ int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int
     workers = resident_pairs(kernel, Cfg::kSmemBytes, dev);
     if (workers <= 0) return static_cast<int>(cudaErrorInvalidConfiguration);
   }
-  if (most_tiles < static_cast<std::uint64_t>(workers)) workers = static_cast<int>(most_tiles);
-  return col::launch_serialised(kernel, dim3(static_cast<unsigned>(workers * CG)),
+  // clusters that share a tile's sum take one tile each
+  if (SPLIT > 1 || most_tiles < static_cast<std::uint64_t>(workers)) {
+    workers = static_cast<int>(most_tiles);
+  }
+  return col::launch_serialised(kernel, dim3(static_cast<unsigned>(workers * CG * SPLIT)),
                                 dim3(col::sm100::kCtaThreads), Cfg::kSmemBytes, s, p);
 }
 
@@ -264,7 +275,7 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   // same for every group, and the sums have T rows over the groups).
   const double used = static_cast<double>(t < experts ? t : experts);
   const double group_rows = static_cast<double>(t) / used;
-  const Variant v = choose_variant(
+  Variant v = choose_variant(
       kBf16Costs,
       [&](int tile_rows) {
         if (MODE == kGradW) return static_cast<double>(experts * ((n + tile_rows - 1) / tile_rows));
@@ -273,10 +284,22 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
       static_cast<double>(out_cols * (SWIGLU ? 2 : 1)),
       MODE == kGradW ? std::ceil(group_rows / 64.0) : static_cast<double>(p.num_k_blocks),
       MODE == kGradW ? 1e9 : group_rows, info.sm_count, MODE != kGradW);
+  if constexpr (MODE != kGradW) {
+    // A few tiles of few rows: four or two CTAs share each sum while there are SMs
+    // for them, with at least four k-blocks apiece.
+    const std::uint64_t tiles = most_row_tiles(t, experts, false, 32) *
+                                ((out_cols * (SWIGLU ? 2 : 1) + 127) / 128);
+    for (const int split : {4, 2}) {
+      if (v.split == 1 && tiles * split <= static_cast<std::uint64_t>(info.sm_count) &&
+          p.num_k_blocks >= 4 * split) {
+        v = Variant{1, 128, 32, split};
+      }
+    }
+  }
   p.num_n_blocks = static_cast<int>((out_cols * (SWIGLU ? 2 : 1) + v.bn - 1) / v.bn);
-  const std::uint64_t tile_rows = static_cast<std::uint64_t>(v.cg * v.rows);
-  const std::uint64_t m_tiles =
-      MODE == kGradW ? experts * ((n + tile_rows - 1) / tile_rows) : t / tile_rows + experts;
+  const int tile_rows = v.cg * v.rows;
+  const std::uint64_t m_tiles = MODE == kGradW ? experts * ((n + tile_rows - 1) / tile_rows)
+                                               : most_row_tiles(t, experts, false, tile_rows);
   const std::uint64_t most_tiles = m_tiles * p.num_n_blocks;
   if (most_tiles > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
   int rc = encode_map(&p.map_a, {a, a_cols, t, 0, MODE == kGradW ? 64u : 128u, 2});
@@ -291,6 +314,8 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   const int sms = info.sm_count;
   if (v.cg == 2) return launch_grouped_bf16<MODE, SWIGLU, 2, 256, 128>(p, most_tiles, dev, sms, s);
   if constexpr (MODE != kGradW) {
+    if (v.split == 4) return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 32, 4>(p, most_tiles, dev, sms, s);
+    if (v.split == 2) return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 32, 2>(p, most_tiles, dev, sms, s);
     if (v.rows == 32) return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 32>(p, most_tiles, dev, sms, s);
   }
   if (v.bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 1, 256, 128>(p, most_tiles, dev, sms, s);
@@ -368,7 +393,7 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
   // SMs for them, with at least two k-blocks apiece.  One row by 4096 x 4096:
   // 12.5 us with one CTA a tile, 9.1 with two, 8.1 with four; one row by 1024 x
   // 4096: 12.2, 8.2, 6.9, and 6.2 with four and 64 columns.
-  const std::uint64_t tiles32 = offsets == nullptr ? (t + 31) / 32 : t / 32 + experts;
+  const std::uint64_t tiles32 = most_row_tiles(t, experts, offsets == nullptr, 32);
   double best_blocks = 0.0;
   for (const int bn : {64, 128}) {
     for (const int split : {2, 4}) {
@@ -383,9 +408,8 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
     }
   }
   p.num_n_blocks = static_cast<int>((w_rows + v.bn - 1) / v.bn);
-  const std::uint64_t tile_rows = static_cast<std::uint64_t>(v.cg * v.rows);
-  const std::uint64_t m_tiles = offsets ? t / tile_rows + experts : (t + tile_rows - 1) / tile_rows;
-  const std::uint64_t most_tiles = m_tiles * p.num_n_blocks;
+  const std::uint64_t most_tiles =
+      most_row_tiles(t, experts, offsets == nullptr, v.cg * v.rows) * p.num_n_blocks;
   if (most_tiles * v.split > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
   int rc = encode_map(&p.map_a, {x, k, t, 0, 128, 1});
   if (rc == 0 && v.cg == 1) rc = encode_map(&p.map_a32, {x, k, t, 0, 32, 1});

@@ -29,6 +29,7 @@
 
 #include "gemm_sm100.cuh"
 #include "gemm_sm100_2sm.cuh"
+#include "gemm_sm100_sk.cuh"
 #include "grouped_schedule.cuh"
 
 namespace col {
@@ -60,18 +61,23 @@ constexpr int b_box_rows(bool swiglu, int cg, int bn) { return swiglu || cg == 2
 // Only those rows of A are loaded and kept (the MMA's other 96 rows read
 // whatever lies behind them; what they add up is not stored), which leaves the
 // ring to w.
-template <int CG, int BN, int ROWS>
+// SPLIT: the CTAs of a cluster share a tile's k-blocks and add their sums up in
+// the first one, for a few tiles of few rows.
+template <int CG, int BN, int ROWS, int SPLIT>
 struct GroupedCfg {
   static_assert(BN == 128 || BN == 256, "tile width");
   static_assert(CG == 1 || CG == 2, "CTAs of a tile");
   static_assert(ROWS == kBlockM || (ROWS == 32 && CG == 1), "rows of a tile");
+  static_assert(SPLIT == 1 || (ROWS == 32 && BN == 128), "shared sums");
   static constexpr int kTileRows = ROWS * CG;
   static constexpr uint32_t kABytes = ROWS * kBlockK * 2;
   static constexpr uint32_t kBBytes = BN / CG * kBlockK * 2;
   static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
   static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : 2;  // k-blocks a stage
   static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
-  static constexpr uint32_t kExtraBytes = 256 + kGroupTableBytes;
+  // 32 rows of 64 sums, from each other CTA, for two warps
+  static constexpr uint32_t kSumBytes = 32 * 64 * 4;
+  static constexpr uint32_t kExtraBytes = 256 + kGroupTableBytes + (SPLIT - 1) * 2 * kSumBytes;
   static constexpr int kStagesFit =
       static_cast<int>((kSmemLimit - 1024 - kExtraBytes) / kStageBytes);
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
@@ -151,6 +157,16 @@ constexpr uint32_t kWarpWaitPolls = 1u << 20;
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 63u) == 0u && *abort_flag) break;
+  }
+  return false;
+}
+
+// warp_wait on data that other CTAs of the cluster wrote.
+__device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity,
+                                                  volatile int* abort_flag) {
+  for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
     if ((i & 63u) == 0u && *abort_flag) break;
   }
   return false;
@@ -307,10 +323,10 @@ __device__ __forceinline__ void store_rows64(const GroupedParams& p, std::size_t
   }
 }
 
-template <int MODE, bool SWIGLU, int CG, int BN, int ROWS>
-__global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
+template <int MODE, bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
+__global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads, 1)
     grouped_bf16_kernel(const __grid_constant__ GroupedParams p) {
-  using Cfg = GroupedCfg<CG, BN, ROWS>;
+  using Cfg = GroupedCfg<CG, BN, ROWS, SPLIT>;
   static_assert(MODE != kGradW || ROWS == kBlockM, "rows of w are not ragged");
   static_assert(MODE == kForward || !SWIGLU, "SwiGLU is a forward epilogue");
   constexpr int kStages = Cfg::kStages;
@@ -330,17 +346,20 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   uint64_t* tempty_bar = tfull_bar + 2;
   uint64_t* drain_bar = tempty_bar + 2;
   uint64_t* tail_bar = drain_bar + 1;  // kStages of them
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tail_bar + kStages);
+  uint64_t* sums_bar = tail_bar + kStages;  // the other CTAs' sums for each of two warps
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sums_bar + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  static_assert((3 * kStages + 5) * 8 + 8 <= 256, "barrier space");
+  static_assert((3 * kStages + 7) * 8 + 8 <= 256, "barrier space");
   const GroupTables tables = group_tables(smem + kStages * Cfg::kStageBytes + 256);
+  uint8_t* other_sums = smem + kStages * Cfg::kStageBytes + 256 + kGroupTableBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
   const bool leader = rank == 0;
-  const int worker = blockIdx.x / CG;
-  const int workers = gridDim.x / CG;
+  const int worker = blockIdx.x / (CG * SPLIT);
+  const int workers = gridDim.x / (CG * SPLIT);  // SPLIT > 1: at least as many as tiles
+  const int share = SPLIT > 1 ? static_cast<int>(cluster_ctarank()) : 0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -354,6 +373,8 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       mbar_init(smem_u32(tempty_bar + a), CG * kEpiWarps);
     }
     mbar_init(smem_u32(drain_bar), 1);
+    mbar_init(smem_u32(sums_bar), 1);
+    mbar_init(smem_u32(sums_bar + 1), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     grid_dependents_launch();
@@ -371,7 +392,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     fill_group_tables(tables, p.offsets, p.groups, p.rows, Cfg::kTileRows, lane);
   }
   tc_fence_before();
-  if constexpr (CG == 2) {
+  if constexpr (CG * SPLIT > 1) {
     cluster_sync();
   } else {
     __syncthreads();
@@ -387,6 +408,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
     num_tiles = p.groups * ((p.out_rows + Cfg::kTileRows - 1) / Cfg::kTileRows) * p.num_n_blocks;
   } else {
     num_tiles = tables.prefix[p.groups] * p.num_n_blocks;
+    if constexpr (SPLIT > 1) num_tiles = min(num_tiles, workers);  // one tile a cluster
   }
 
   if (warp == 0) {
@@ -409,13 +431,15 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       const int rows = min(ROWS, (t.end - t.a_row + 31) & ~31);
       const bool whole = MODE == kGradW || CG == 2 || rows == kBlockM;
       const bool ragged = MODE == kGradW && ragged_rows(t) != 0;
-      for (int kb = 0; kb < t.k_blocks; kb += kKps) {
+      const int kb_begin = t.k_blocks * share / SPLIT;
+      const int kb_end = t.k_blocks * (share + 1) / SPLIT;
+      for (int kb = kb_begin; kb < kb_end; kb += kKps) {
         if (filled >= kStages && !warp_wait(smem_u32(empty_bar + stage), phase ^ 1u, abort_flag)) {
           if (lane == 0) fail(kStatusProducer);
           ok = false;
           break;
         }
-        const int nk = min(kKps, t.k_blocks - kb);
+        const int nk = min(kKps, kb_end - kb);
         if (elect_one()) {
           const uint32_t bytes = nk * ((whole ? Cfg::kABytes : rows * 128u) + Cfg::kBBytes);
           const uint32_t fb_local = smem_u32(full_bar + stage);
@@ -519,14 +543,16 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + acc * BN;
         const int last_rows = MODE == kGradW ? t.end - t.begin - (t.k_blocks - 1) * kBlockK : 0;
-        for (int kb = 0; kb < t.k_blocks; kb += kKps) {
+        const int kb_begin = t.k_blocks * share / SPLIT;
+        const int kb_end = t.k_blocks * (share + 1) / SPLIT;
+        for (int kb = kb_begin; kb < kb_end; kb += kKps) {
           if (!warp_wait(smem_u32(full_bar + stage), phase, abort_flag)) {
             if (lane == 0) fail(kStatusMma);
             ok = false;
             break;
           }
           tc_fence_after();
-          const int nk = min(kKps, t.k_blocks - kb);
+          const int nk = min(kKps, kb_end - kb);
           if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < kKps; ++j) {
@@ -542,7 +568,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
                                                    : sdesc_kmajor_sw128(sa + k * 32);
                 const uint64_t bd = MODE == kForward ? sdesc_kmajor_sw128(sb + k * 32)
                                                      : sdesc_mnmajor_sw128(sb + k * 2048, kChunkBytes);
-                const uint32_t accumulate = (kb + j != 0 || k != 0) ? 1u : 0u;
+                const uint32_t accumulate = (kb + j != kb_begin || k != 0) ? 1u : 0u;
                 if constexpr (CG == 2) {
                   umma_bf16_pair(d_tmem, ad, bd, kIdesc, accumulate);
                 } else {
@@ -651,7 +677,74 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
       ++local;
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
-      if (valid > 0) {
+      if constexpr (SPLIT > 1) {
+        // This warp's 64 sums a row, 32 at a time: of its columns, or gate and up
+        // ones of the same outputs.  The first CTA adds the others' in their order;
+        // words j .. j + 3 of chunk i lie at (i * 8 + j / 4) * 512 + lane * 16, whole
+        // rows of banks for both sides.
+        auto chunk = [&](int i) { return t_row + mine + (SWIGLU ? i * (BN / 2) : i * 32); };
+        bool got = true;
+        if (valid > 0 && share != 0) {
+          const uint32_t to =
+              map_to_cta(smem_u32(other_sums + ((share - 1) * 2 + half) * Cfg::kSumBytes), 0) + lane * 16;
+          const uint32_t bar = map_to_cta(smem_u32(sums_bar + half), 0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t a[32];
+            tmem_ld32(chunk(i), a);
+            if (lane < valid) {
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                st_async_v4(to + (i * 8 + j / 4) * 512, a[j], a[j + 1], a[j + 2], a[j + 3], bar);
+              }
+            }
+          }
+        } else if (valid > 0) {
+          const uint32_t bar = smem_u32(sums_bar + half);
+          if (lane == 0) mbar_arrive_expect_tx(bar, (SPLIT - 1) * valid * 64 * 4);
+          __syncwarp();
+          got = warp_wait_cluster(bar, 0, abort_flag);
+          if (got) {
+            float f[2][32];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              uint32_t a[32];
+              tmem_ld32(chunk(i), a);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) f[i][j] = __uint_as_float(a[j]);
+              // rows behind the last one read what lies there, and are not stored
+#pragma unroll 1
+              for (int from = 0; from < SPLIT - 1; ++from) {
+                const uint8_t* src = other_sums + (from * 2 + half) * Cfg::kSumBytes + lane * 16;
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                  const float4 v = *reinterpret_cast<const float4*>(src + (i * 8 + j / 4) * 512);
+                  f[i][j] += v.x;
+                  f[i][j + 1] += v.y;
+                  f[i][j + 2] += v.z;
+                  f[i][j + 3] += v.w;
+                }
+              }
+            }
+            uint32_t w[32];
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              if constexpr (SWIGLU) {
+                w[j / 2] = pack_bf16x2(silu_fast(f[0][j]) * f[1][j], silu_fast(f[0][j + 1]) * f[1][j + 1]);
+                w[16 + j / 2] = 0u;
+              } else {
+                w[j / 2] = pack_bf16x2(f[0][j], f[0][j + 1]);
+                w[16 + j / 2] = pack_bf16x2(f[1][j], f[1][j + 1]);
+              }
+            }
+            store_rows64(p, out_row, valid, t.col + mine, kRun, w, lane);
+          }
+        }
+        if (!got) {
+          if (lane == 0) fail(kStatusEpilogue);
+          break;
+        }
+      } else if (valid > 0) {
 #pragma unroll 1
         for (int c = mine; c < mine + kMine; c += kRun) {
           uint32_t w[32];
@@ -692,7 +785,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kCtaThreads, 1)
   // No CTA leaves while its partner may still address its shared memory.
   __syncwarp();
   tc_fence_before();
-  if constexpr (CG == 2) {
+  if constexpr (CG * SPLIT > 1) {
     cluster_sync();
   } else {
     __syncthreads();

@@ -76,7 +76,9 @@ def test_forward_swiglu(name, n, k):
 TILES = [([300, 513, 0, 129], 136, 144), ([300, 513, 0, 129], 2000, 144),
          ([300, 513, 0, 129], 136, 2064), ([700, 0, 650], 2000, 2064), ([700, 0, 650], 1000, 2064),
          ([100] * 16, 136, 144), ([90, 70, 0, 110, 128, 60], 1000, 528),
-         ([20] * 10, 264, 2064), ([5, 0, 40, 3], 264, 2064)]
+         ([20] * 10, 264, 2064), ([5, 0, 40, 3], 264, 2064),
+         # gradients whose sums the CTAs of a cluster share
+         ([5, 0, 40, 3], 1032, 136), ([20] * 10, 1032, 264), ([1, 0, 1], 4104, 520)]
 
 
 def pairs_of(lengths):
