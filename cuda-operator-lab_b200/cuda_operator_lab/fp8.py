@@ -131,12 +131,17 @@ def quantize_fp8_block128_into(x: torch.Tensor, q: torch.Tensor,
 
 def quantize_fp8_block128(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Allocating form of :func:`quantize_fp8_block128_into`: ``(q, scale)``."""
-    m, k = _check_rows(x)
-    _check_placement("FP8 quantize", x)
+    symbol = _ROWS.get(x.dtype)
+    if symbol is None or x.ndim != 2 or not x.is_cuda or not x.is_contiguous():
+        _check_rows(x)
+        _check_placement("FP8 quantize", x)
+    m, k = x.shape
+    if m > _MAX_SIZE or k > _MAX_SIZE:
+        _check_sizes("FP8 quantize", m, k)
     q = torch.empty_like(x, dtype=_E4M3)
-    scale = x.new_empty((m, _blocks(k)), dtype=torch.float32)
+    scale = torch.empty(m, _blocks(k), device=x.device, dtype=torch.float32)
     if m and k:
-        _launch(_ROWS[x.dtype], x, _ptr(x), _ptr(q), _ptr(scale), m, k)
+        _launch(symbol, x, x.data_ptr(), q.data_ptr(), scale.data_ptr(), m, k)
     return q, scale
 
 
@@ -233,7 +238,7 @@ def _gemm(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: 
     m, k, n = _check_fp8_operands(what, x_fp8, x_scale, weight_fp8, weight_scale, swiglu)
     if out is None:
         _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale)
-        out = x_fp8.new_empty((m, n), dtype=torch.bfloat16)
+        out = torch.empty(m, n, device=x_fp8.device, dtype=torch.bfloat16)
     else:
         _check_output(what, out, (m, n))
         _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, out)

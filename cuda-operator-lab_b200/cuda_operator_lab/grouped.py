@@ -57,6 +57,10 @@ def _check_bf16(what: str, *tensors: torch.Tensor) -> None:
             raise TypeError(f"{what} expects bfloat16 tensors")
 
 
+def _new(on: torch.Tensor, *shape: int) -> torch.Tensor:
+    return torch.empty(*shape, device=on.device, dtype=torch.bfloat16)
+
+
 def _check_ranks(x: torch.Tensor, weight: torch.Tensor) -> None:
     if x.ndim != 2 or weight.ndim != 3:
         raise ValueError("x must be 2-D and weight 3-D")
@@ -96,7 +100,7 @@ def _forward(swiglu: bool, x: torch.Tensor, weight: torch.Tensor, offsets: torch
     t, k, n, experts = _check_forward(what, swiglu, x, weight, offsets)
     if out is None:
         _check_placement(what, x, weight, offsets)
-        out = x.new_empty((t, n))
+        out = _new(x, t, n)
     else:
         _check_output(what, out, (t, n))
         _check_placement(what, x, weight, offsets, out)
@@ -174,8 +178,7 @@ def gemm_grouped_bf16_grad_input(grad_bf16: torch.Tensor, weight_bf16: torch.Ten
     """Allocating form of :func:`gemm_grouped_bf16_grad_input_into`."""
     t, k, n, experts = _check_grad_input(grad_bf16, weight_bf16, offsets)
     _check_placement(_GRAD, grad_bf16, weight_bf16, offsets)
-    return _run_grad_input(grad_bf16, weight_bf16, offsets, grad_bf16.new_empty((t, k)), t, k, n,
-                           experts)
+    return _run_grad_input(grad_bf16, weight_bf16, offsets, _new(grad_bf16, t, k), t, k, n, experts)
 
 
 def _check_grad_weight(grad: torch.Tensor, x: torch.Tensor,
@@ -222,7 +225,7 @@ def gemm_grouped_bf16_grad_weight(grad_bf16: torch.Tensor, x_bf16: torch.Tensor,
     """Allocating form of :func:`gemm_grouped_bf16_grad_weight_into`."""
     t, k, n, experts = _check_grad_weight(grad_bf16, x_bf16, offsets)
     _check_placement(_GRAD, grad_bf16, x_bf16, offsets)
-    return _run_grad_weight(grad_bf16, x_bf16, offsets, grad_bf16.new_empty((experts, n, k)), t, k,
+    return _run_grad_weight(grad_bf16, x_bf16, offsets, _new(grad_bf16, experts, n, k), t, k,
                             n, experts)
 
 
@@ -235,9 +238,9 @@ def gemm_grouped_bf16_backward(grad_bf16: torch.Tensor, x_bf16: torch.Tensor,
         raise ValueError(f"x shape must be {(t, k)}")
     _check_bf16(_GRAD, x_bf16)
     _check_placement(_GRAD, grad_bf16, x_bf16, weight_bf16, offsets)
-    return (_run_grad_input(grad_bf16, weight_bf16, offsets, grad_bf16.new_empty((t, k)), t, k, n,
+    return (_run_grad_input(grad_bf16, weight_bf16, offsets, _new(grad_bf16, t, k), t, k, n,
                             experts),
-            _run_grad_weight(grad_bf16, x_bf16, offsets, grad_bf16.new_empty((experts, n, k)), t,
+            _run_grad_weight(grad_bf16, x_bf16, offsets, _new(grad_bf16, experts, n, k), t,
                              k, n, experts))
 
 
@@ -254,7 +257,7 @@ def _fp8(swiglu: bool, x_fp8: torch.Tensor, x_scale: torch.Tensor, weight_fp8: t
     _check_offsets(what, offsets, experts)
     if out is None:
         _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, offsets)
-        out = x_fp8.new_empty((t, n), dtype=torch.bfloat16)
+        out = _new(x_fp8, t, n)
     else:
         _check_output(what, out, (t, n))
         _check_placement(what, x_fp8, x_scale, weight_fp8, weight_scale, offsets, out)
