@@ -245,18 +245,14 @@ int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int
                                 dim3(col::sm100::kCtaThreads), Cfg::kSmemBytes, s, p);
 }
 
-// Tensor-core product; -1 where TMA cannot address the operands.
+// What a product's kernel gets, but for its tiles; -1 where TMA cannot address the
+// operands.
 template <int MODE, bool SWIGLU>
-int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, void* out,
-                    std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
-                    cudaStream_t s) {
-  const std::uint64_t w_rows = SWIGLU ? 2 * n : n;
-  const std::uint64_t a_cols = MODE == kForward ? k : n;
-  if (!tma_ok(a, a_cols, 2) || !tma_ok(b, k, 2)) return -1;
-  int dev = 0;
-  const col::DeviceInfo& info = col::device_info(&dev);
+int grouped_params(GroupedParams& p, const void* a, const void* b, const std::int32_t* offsets,
+                   void* out, std::uint64_t t, std::uint64_t k, std::uint64_t n,
+                   std::uint64_t experts, int dev, const col::DeviceInfo& info) {
+  if (!tma_ok(a, MODE == kForward ? k : n, 2) || !tma_ok(b, k, 2)) return -1;
   if (info.cc_major != 10) return col::kErrDeviceNotSupported;
-  GroupedParams p;
   std::memset(&p, 0, sizeof(p));
   p.status = col::gemm_status_ptr(dev);
   if (!p.status) return static_cast<int>(cudaErrorInvalidDevice);
@@ -270,7 +266,36 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   p.num_k_blocks = static_cast<int>(((MODE == kForward ? k : n) + 63) / 64);
   p.up_offset = static_cast<int>(n);
   p.out_vec_ok = col::aligned16(out) && out_cols % 8 == 0;
+  return 0;
+}
 
+// The column tiles and tensor maps of a variant.
+template <int MODE, bool SWIGLU>
+int grouped_maps(GroupedParams& p, const Variant& v, const void* a, const void* b, std::uint64_t t,
+                 std::uint64_t k, std::uint64_t n, std::uint64_t experts) {
+  const std::uint64_t a_cols = MODE == kForward ? k : n;
+  p.num_n_blocks = (p.out_cols * (SWIGLU ? 2 : 1) + v.bn - 1) / v.bn;
+  int rc = encode_map(&p.map_a, {a, a_cols, t, 0, MODE == kGradW ? 64u : 128u, 2});
+  if (rc == 0 && MODE != kGradW && v.cg == 1) rc = encode_map(&p.map_a32, {a, a_cols, t, 0, 32, 2});
+  if (rc != 0) return rc;
+  const std::uint32_t b_box =
+      MODE == kForward ? static_cast<std::uint32_t>(col::sm100::b_box_rows(SWIGLU, v.cg, v.bn)) : 64u;
+  return MODE == kGradW
+             ? encode_map(&p.map_b, {b, k, t, 0, b_box, 2})
+             : encode_map(&p.map_b, {b, k, SWIGLU ? 2 * n : n, experts, b_box, 2});
+}
+
+// Tensor-core product; -1 where TMA cannot address the operands.
+template <int MODE, bool SWIGLU>
+int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, void* out,
+                    std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
+                    cudaStream_t s) {
+  int dev = 0;
+  const col::DeviceInfo& info = col::device_info(&dev);
+  GroupedParams p;
+  int rc = grouped_params<MODE, SWIGLU>(p, a, b, offsets, out, t, k, n, experts, dev, info);
+  if (rc != 0) return rc;
+  const std::uint64_t out_cols = MODE == kForward ? n : k;
   // Rows a group: of the operand that a tile's rows come from (kGradW: of w, the
   // same for every group, and the sums have T rows over the groups).
   const double used = static_cast<double>(t < experts ? t : experts);
@@ -296,21 +321,13 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
       }
     }
   }
-  p.num_n_blocks = static_cast<int>((out_cols * (SWIGLU ? 2 : 1) + v.bn - 1) / v.bn);
+  rc = grouped_maps<MODE, SWIGLU>(p, v, a, b, t, k, n, experts);
+  if (rc != 0) return rc;
   const int tile_rows = v.cg * v.rows;
   const std::uint64_t m_tiles = MODE == kGradW ? experts * ((n + tile_rows - 1) / tile_rows)
                                                : most_row_tiles(t, experts, false, tile_rows);
   const std::uint64_t most_tiles = m_tiles * p.num_n_blocks;
   if (most_tiles > kIntMax) return static_cast<int>(cudaErrorInvalidValue);
-  int rc = encode_map(&p.map_a, {a, a_cols, t, 0, MODE == kGradW ? 64u : 128u, 2});
-  if (rc == 0 && MODE != kGradW && v.cg == 1) rc = encode_map(&p.map_a32, {a, a_cols, t, 0, 32, 2});
-  if (rc == 0) {
-    const std::uint32_t b_box =
-        MODE == kForward ? static_cast<std::uint32_t>(col::sm100::b_box_rows(SWIGLU, v.cg, v.bn)) : 64u;
-    rc = MODE == kGradW ? encode_map(&p.map_b, {b, k, t, 0, b_box, 2})
-                        : encode_map(&p.map_b, {b, k, w_rows, experts, b_box, 2});
-  }
-  if (rc != 0) return rc;
   const int sms = info.sm_count;
   if (v.cg == 2) return launch_grouped_bf16<MODE, SWIGLU, 2, 256, 128>(p, most_tiles, dev, sms, s);
   if constexpr (MODE != kGradW) {
@@ -320,6 +337,43 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   }
   if (v.bn == 256) return launch_grouped_bf16<MODE, SWIGLU, 1, 256, 128>(p, most_tiles, dev, sms, s);
   return launch_grouped_bf16<MODE, SWIGLU, 1, 128, 128>(p, most_tiles, dev, sms, s);
+}
+
+template <int ROWS>
+int launch_backward(const GroupedParams& by_x, const GroupedParams& by_w, int input_ctas,
+                    int weight_ctas, int dev, cudaStream_t s) {
+  constexpr std::uint32_t kX = GroupedCfg<1, 128, ROWS, 1>::kSmemBytes;
+  constexpr std::uint32_t kW = GroupedCfg<1, 128, 128, 1>::kSmemBytes;
+  constexpr std::uint32_t kSmem = kX > kW ? kX : kW;
+  auto kernel = col::sm100::grouped_bf16_backward_kernel<ROWS>;
+  static std::atomic<std::uint64_t> done{0};
+  if (int rc = allow_smem(kernel, kSmem, dev, done)) return rc;
+  return col::launch_serialised(kernel, dim3(static_cast<unsigned>(input_ctas + weight_ctas)),
+                                dim3(col::sm100::kCtaThreads), kSmem, s, by_x, by_w, input_ctas);
+}
+
+// Both gradients in one launch where the tiles of both have an SM each; -1 where
+// they do not, or TMA cannot address the operands.
+int backward_tc(const void* grad, const void* x, const void* w, const std::int32_t* offsets,
+                void* dx, void* dw, std::uint64_t t, std::uint64_t k, std::uint64_t n,
+                std::uint64_t experts, cudaStream_t s) {
+  int dev = 0;
+  const col::DeviceInfo& info = col::device_info(&dev);
+  const std::uint64_t columns = (k + 127) / 128;
+  const int rows = t <= 32 * experts ? 32 : 128;
+  const std::uint64_t input_tiles = most_row_tiles(t, experts, false, rows) * columns;
+  const std::uint64_t weight_tiles = experts * ((n + 127) / 128) * columns;
+  if (input_tiles + weight_tiles > static_cast<std::uint64_t>(info.sm_count)) return -1;
+  GroupedParams by_x, by_w;
+  int rc = grouped_params<kGradX, false>(by_x, grad, w, offsets, dx, t, k, n, experts, dev, info);
+  if (rc == 0) rc = grouped_params<kGradW, false>(by_w, grad, x, offsets, dw, t, k, n, experts, dev, info);
+  if (rc == 0) rc = grouped_maps<kGradX, false>(by_x, {1, 128, rows, 1}, grad, w, t, k, n, experts);
+  if (rc == 0) rc = grouped_maps<kGradW, false>(by_w, {1, 128, 128, 1}, grad, x, t, k, n, experts);
+  if (rc != 0) return rc;
+  const int input_ctas = static_cast<int>(input_tiles);
+  const int weight_ctas = static_cast<int>(weight_tiles);
+  if (rows == 32) return launch_backward<32>(by_x, by_w, input_ctas, weight_ctas, dev, s);
+  return launch_backward<128>(by_x, by_w, input_ctas, weight_ctas, dev, s);
 }
 
 template <bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
@@ -528,6 +582,27 @@ COL_API int cuda_operator_gemm_grouped_bf16_grad_weight(const void* grad_bf16,
   const GroupedSimtParams p =
       simt_params(grad_bf16, input_bf16, offsets, grad_weight_bf16, t, k, n, n, experts);
   return col::simt::launch_grouped_simt<__nv_bfloat16, col::simt::kGradW, false>(p, s);
+}
+
+COL_API int cuda_operator_gemm_grouped_bf16_backward(const void* grad_bf16, const void* input_bf16,
+                                                     const void* weight_bf16,
+                                                     const int32_t* offsets, void* grad_input_bf16,
+                                                     void* grad_weight_bf16, uint64_t t, uint64_t k,
+                                                     uint64_t n, uint64_t experts, void* stream) {
+  if (t != 0 && k != 0 && n != 0 && experts != 0) {
+    if (!grad_bf16 || !input_bf16 || !weight_bf16 || !offsets || !grad_input_bf16 ||
+        !grad_weight_bf16 || !sizes_ok(t, k, n, experts)) {
+      return static_cast<int>(cudaErrorInvalidValue);
+    }
+    const int rc = backward_tc(grad_bf16, input_bf16, weight_bf16, offsets, grad_input_bf16,
+                               grad_weight_bf16, t, k, n, experts, col::as_stream(stream));
+    if (rc != -1) return rc;
+  }
+  const int rc = cuda_operator_gemm_grouped_bf16_grad_input(
+      grad_bf16, weight_bf16, offsets, grad_input_bf16, t, k, n, experts, stream);
+  if (rc != 0) return rc;
+  return cuda_operator_gemm_grouped_bf16_grad_weight(grad_bf16, input_bf16, offsets,
+                                                     grad_weight_bf16, t, k, n, experts, stream);
 }
 
 COL_API int cuda_operator_gemm_fp8_block128(const void* input_fp8, const float* input_scale,

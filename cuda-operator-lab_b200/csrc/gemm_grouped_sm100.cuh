@@ -323,9 +323,10 @@ __device__ __forceinline__ void store_rows64(const GroupedParams& p, std::size_t
   }
 }
 
+// One CTA of a product; worker w of `workers` (CTAs, pairs or clusters) takes tiles
+// w, w + workers, ...; SPLIT > 1: there are at least as many workers as tiles.
 template <int MODE, bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
-__global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads, 1)
-    grouped_bf16_kernel(const __grid_constant__ GroupedParams p) {
+__device__ __forceinline__ void grouped_bf16_cta(const GroupedParams& p, int worker, int workers) {
   using Cfg = GroupedCfg<CG, BN, ROWS, SPLIT>;
   static_assert(MODE != kGradW || ROWS == kBlockM, "rows of w are not ragged");
   static_assert(MODE == kForward || !SWIGLU, "SwiGLU is a forward epilogue");
@@ -357,8 +358,6 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
   const int lane = threadIdx.x & 31;
   const int rank = CG == 2 ? static_cast<int>(cluster_ctarank()) : 0;
   const bool leader = rank == 0;
-  const int worker = blockIdx.x / (CG * SPLIT);
-  const int workers = gridDim.x / (CG * SPLIT);  // SPLIT > 1: at least as many as tiles
   const int share = SPLIT > 1 ? static_cast<int>(cluster_ctarank()) : 0;
 
   if (threadIdx.x == 0) {
@@ -797,6 +796,28 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
     } else {
       tmem_dealloc(tmem_base, Cfg::kTmemCols);
     }
+  }
+}
+
+template <int MODE, bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
+__global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads, 1)
+    grouped_bf16_kernel(const __grid_constant__ GroupedParams p) {
+  grouped_bf16_cta<MODE, SWIGLU, CG, BN, ROWS, SPLIT>(p, blockIdx.x / (CG * SPLIT),
+                                                      gridDim.x / (CG * SPLIT));
+}
+
+// Both gradients of a small product in one launch, side by side: the first
+// input_ctas CTAs compute the one by x, the others the one by W.
+template <int ROWS>
+__global__ void __launch_bounds__(kCtaThreads, 1)
+    grouped_bf16_backward_kernel(const __grid_constant__ GroupedParams by_x,
+                                 const __grid_constant__ GroupedParams by_w, int input_ctas) {
+  const int cta = blockIdx.x;
+  if (cta < input_ctas) {
+    grouped_bf16_cta<kGradX, false, 1, 128, ROWS, 1>(by_x, cta, input_ctas);
+  } else {
+    grouped_bf16_cta<kGradW, false, 1, 128, kBlockM, 1>(by_w, cta - input_ctas,
+                                                        gridDim.x - input_ctas);
   }
 }
 

@@ -100,6 +100,8 @@ for _v in ("gemm_grouped", "gemm_grouped_swiglu"):
     _SIGNATURES[f"cuda_operator_{_v}_bf16"] = [_P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]
     _SIGNATURES[f"cuda_operator_{_v}_fp8_block128"] = [
         _P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]
+_SIGNATURES["cuda_operator_gemm_grouped_bf16_backward"] = [
+    _P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]
 for _v in ("input", "weight"):
     _SIGNATURES[f"cuda_operator_gemm_grouped_bf16_grad_{_v}"] = [
         _P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]

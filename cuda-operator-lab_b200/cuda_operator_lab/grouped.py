@@ -238,10 +238,13 @@ def gemm_grouped_bf16_backward(grad_bf16: torch.Tensor, x_bf16: torch.Tensor,
         raise ValueError(f"x shape must be {(t, k)}")
     _check_bf16(_GRAD, x_bf16)
     _check_placement(_GRAD, grad_bf16, x_bf16, weight_bf16, offsets)
-    return (_run_grad_input(grad_bf16, weight_bf16, offsets, _new(grad_bf16, t, k), t, k, n,
-                            experts),
-            _run_grad_weight(grad_bf16, x_bf16, offsets, _new(grad_bf16, experts, n, k), t,
-                             k, n, experts))
+    grad_input = _new(grad_bf16, t, k)
+    grad_weight = _new(grad_bf16, experts, n, k)
+    if k and experts:
+        _launch("cuda_operator_gemm_grouped_bf16_backward", grad_bf16, _ptr(grad_bf16),
+                _ptr(x_bf16), _ptr(weight_bf16), _ptr(offsets), _ptr(grad_input),
+                _ptr(grad_weight), t, k, n, experts)
+    return grad_input, grad_weight
 
 
 # ---------------------------------------------------------------- block-scaled e4m3

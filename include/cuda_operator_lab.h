@@ -329,6 +329,9 @@ int cuda_operator_gemm_grouped_swiglu_fp8_block128(const void* input_fp8, const 
 int cuda_operator_gemm_grouped_bf16_grad_input(const void* grad_bf16, const void* weight_bf16, const int32_t* offsets, void* grad_input_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
 int cuda_operator_gemm_grouped_bf16_grad_weight(const void* grad_bf16, const void* input_bf16, const int32_t* offsets, void* grad_weight_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
 
+/* Both of them, in one launch where the product is small. */
+int cuda_operator_gemm_grouped_bf16_backward(const void* grad_bf16, const void* input_bf16, const void* weight_bf16, const int32_t* offsets, void* grad_input_bf16, void* grad_weight_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
+
 /* Number of SMs of the current device and the library's build tag; lets a
  * caller check which library it loaded.  Host-only, enqueues nothing. */
 int cuda_operator_lab_device_info(int* sm_count, int* cc_major, int* cc_minor);

@@ -187,6 +187,14 @@ def test_c_entries_refuse_bad_sizes_and_pointers():
         "dx": lambda *a: lib.cuda_operator_gemm_grouped_bf16_grad_input(*a, None),
         "dw": lambda *a: lib.cuda_operator_gemm_grouped_bf16_grad_weight(*a, None),
     }
+    call["both"] = lambda *a: lib.cuda_operator_gemm_grouped_bf16_backward(*a, None)
+    for null in range(6):
+        args = [p] * 6
+        args[null] = None
+        assert call["both"](*args, 4, 8, 8, 2) == invalid, null
+    assert call["both"](*[p] * 6, 1 << 31, 8, 8, 2) == invalid
+    assert call["both"](*[p] * 6, 4, 8, 8, 1025) == invalid
+    assert call["both"](*[None] * 6, 0, 0, 8, 2) == 0
     # nothing to do succeeds before any check
     assert call["quantize"](None, None, None, 0, 8) == 0
     assert call["tiles"](None, None, None, 0, 8, 8) == 0
