@@ -205,7 +205,8 @@ std::uint64_t most_row_tiles(std::uint64_t rows, std::uint64_t groups, bool know
 // `columns` (accumulator columns) span the tiles, `k_blocks` the sum of one.
 template <int COUNT, typename RowTiles>
 Variant choose_variant(const VariantCost (&costs)[COUNT], RowTiles row_tiles, double columns,
-                       double k_blocks, double rows_per_group, int sm_count, bool rows32) {
+                       double k_blocks, double rows_per_group, int sm_count, bool rows32,
+                       double* us_out = nullptr) {
   Variant best = costs[0].v;
   double best_us = -1.0;
   for (const VariantCost& c : costs) {
@@ -222,6 +223,7 @@ Variant choose_variant(const VariantCost (&costs)[COUNT], RowTiles row_tiles, do
       best_us = us;
     }
   }
+  if (us_out) *us_out = best_us;
   return best;
 }
 
@@ -243,6 +245,26 @@ int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int
   }
   return col::launch_serialised(kernel, dim3(static_cast<unsigned>(workers * CG * SPLIT)),
                                 dim3(col::sm100::kCtaThreads), Cfg::kSmemBytes, s, p);
+}
+
+// The variant of a bf16 product with `columns` accumulator columns, and its time.
+template <int MODE>
+Variant choose_bf16(std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
+                    std::uint64_t columns, int sm_count, double* us_out = nullptr) {
+  // Rows a group: of the operand that a tile's rows come from (kGradW: of w, the
+  // same for every group, and the sums have T rows over the groups).
+  const double group_rows = static_cast<double>(t) / static_cast<double>(t < experts ? t : experts);
+  const double k_blocks = MODE == kGradW   ? std::ceil(group_rows / 64.0)
+                          : MODE == kGradX ? std::ceil(static_cast<double>(n) / 64.0)
+                                           : std::ceil(static_cast<double>(k) / 64.0);
+  return choose_variant(
+      kBf16Costs,
+      [&](int tile_rows) {
+        if (MODE == kGradW) return static_cast<double>(experts * ((n + tile_rows - 1) / tile_rows));
+        return expected_row_tiles(t, experts, false, tile_rows);
+      },
+      static_cast<double>(columns), k_blocks, MODE == kGradW ? 1e9 : group_rows, sm_count,
+      MODE != kGradW, us_out);
 }
 
 // What a product's kernel gets, but for its tiles; -1 where TMA cannot address the
@@ -296,19 +318,7 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   int rc = grouped_params<MODE, SWIGLU>(p, a, b, offsets, out, t, k, n, experts, dev, info);
   if (rc != 0) return rc;
   const std::uint64_t out_cols = MODE == kForward ? n : k;
-  // Rows a group: of the operand that a tile's rows come from (kGradW: of w, the
-  // same for every group, and the sums have T rows over the groups).
-  const double used = static_cast<double>(t < experts ? t : experts);
-  const double group_rows = static_cast<double>(t) / used;
-  Variant v = choose_variant(
-      kBf16Costs,
-      [&](int tile_rows) {
-        if (MODE == kGradW) return static_cast<double>(experts * ((n + tile_rows - 1) / tile_rows));
-        return expected_row_tiles(t, experts, false, tile_rows);
-      },
-      static_cast<double>(out_cols * (SWIGLU ? 2 : 1)),
-      MODE == kGradW ? std::ceil(group_rows / 64.0) : static_cast<double>(p.num_k_blocks),
-      MODE == kGradW ? 1e9 : group_rows, info.sm_count, MODE != kGradW);
+  Variant v = choose_bf16<MODE>(t, k, n, experts, SWIGLU ? 2 * out_cols : out_cols, info.sm_count);
   if constexpr (MODE != kGradW) {
     // A few tiles of few rows: four or two CTAs share each sum while there are SMs
     // for them, with at least four k-blocks apiece.
@@ -352,8 +362,16 @@ int launch_backward(const GroupedParams& by_x, const GroupedParams& by_w, int in
                                 dim3(col::sm100::kCtaThreads), kSmem, s, by_x, by_w, input_ctas);
 }
 
-// Both gradients in one launch where the tiles of both have an SM each; -1 where
-// they do not, or TMA cannot address the operands.
+// Both gradients in one launch, each on its share of the SMs, where that takes
+// less than two launches after one another; -1 where it does not, or TMA cannot
+// address the operands.  A second launch costs kSecondLaunchUs on the GPU (its
+// start, and the first one's last wave), and ~6 us of the caller's time.
+// 1100 rows over 20 experts, 520 x 776: 21.6 -> 16.6 us; 14 over 28, 216 x 184: 10.4
+// -> 5.5.  The margin is for shares that uneven groups unbalance: without it 3519
+// rows over 5, 2264 x 568, took 50.6 us instead of 39.6.
+constexpr double kSecondLaunchUs = 4.0;
+constexpr double kBothMargin = 1.2;
+
 int backward_tc(const void* grad, const void* x, const void* w, const std::int32_t* offsets,
                 void* dx, void* dw, std::uint64_t t, std::uint64_t k, std::uint64_t n,
                 std::uint64_t experts, cudaStream_t s) {
@@ -361,17 +379,34 @@ int backward_tc(const void* grad, const void* x, const void* w, const std::int32
   const col::DeviceInfo& info = col::device_info(&dev);
   const std::uint64_t columns = (k + 127) / 128;
   const int rows = t <= 32 * experts ? 32 : 128;
-  const std::uint64_t input_tiles = most_row_tiles(t, experts, false, rows) * columns;
-  const std::uint64_t weight_tiles = experts * ((n + 127) / 128) * columns;
-  if (input_tiles + weight_tiles > static_cast<std::uint64_t>(info.sm_count)) return -1;
+  const double group_rows = static_cast<double>(t) / static_cast<double>(t < experts ? t : experts);
+  const double input_tiles = expected_row_tiles(t, experts, false, rows) * static_cast<double>(columns);
+  const double weight_tiles = static_cast<double>(experts * ((n + 127) / 128) * columns);
+  // a tile's time in either, as in kBf16Costs
+  const double input_us = std::ceil(static_cast<double>(n) / 64.0) * 0.3 + 0.8;
+  const double weight_us = std::ceil(group_rows / 64.0) * 0.285 + 0.8;
+  double input_share = input_tiles;
+  double weight_share = weight_tiles;
+  if (input_tiles + weight_tiles > info.sm_count) {
+    const double part = input_tiles * input_us / (input_tiles * input_us + weight_tiles * weight_us);
+    input_share = std::fmin(std::fmax(std::round(part * info.sm_count), 1.0), info.sm_count - 1.0);
+    weight_share = info.sm_count - input_share;
+  }
+  const double both_us = std::fmax(std::ceil(input_tiles / input_share) * input_us,
+                                   std::ceil(weight_tiles / weight_share) * weight_us);
+  double first_us = 0.0;
+  double second_us = 0.0;
+  choose_bf16<kGradX>(t, k, n, experts, k, info.sm_count, &first_us);
+  choose_bf16<kGradW>(t, k, n, experts, k, info.sm_count, &second_us);
+  if (both_us * kBothMargin >= first_us + second_us + kSecondLaunchUs) return -1;
   GroupedParams by_x, by_w;
   int rc = grouped_params<kGradX, false>(by_x, grad, w, offsets, dx, t, k, n, experts, dev, info);
   if (rc == 0) rc = grouped_params<kGradW, false>(by_w, grad, x, offsets, dw, t, k, n, experts, dev, info);
   if (rc == 0) rc = grouped_maps<kGradX, false>(by_x, {1, 128, rows, 1}, grad, w, t, k, n, experts);
   if (rc == 0) rc = grouped_maps<kGradW, false>(by_w, {1, 128, 128, 1}, grad, x, t, k, n, experts);
   if (rc != 0) return rc;
-  const int input_ctas = static_cast<int>(input_tiles);
-  const int weight_ctas = static_cast<int>(weight_tiles);
+  const int input_ctas = static_cast<int>(std::ceil(input_share));
+  const int weight_ctas = static_cast<int>(weight_share);
   if (rows == 32) return launch_backward<32>(by_x, by_w, input_ctas, weight_ctas, dev, s);
   return launch_backward<128>(by_x, by_w, input_ctas, weight_ctas, dev, s);
 }

@@ -193,6 +193,29 @@ def test_backward_of_long_sums(lengths):
         em.assert_within(dw[e].cpu(), *em.product(gr.mT, xr.mT, False))
 
 
+@pytest.mark.parametrize("lengths,n,k", [([3, 0, 9, 2], 184, 216), ([200, 31, 0], 320, 200),
+                                         ([70, 0, 5, 130] * 5, 776, 520), ([2] * 60, 384, 160),
+                                         ([400, 333, 64], 2000, 1032), ([0, 0], 64, 64)])
+def test_both_gradients_are_those_of_their_own_calls(lengths, n, k):
+    """In one launch side by side or after one another; some rows of no expert."""
+    t, off = sum(lengths) + 9, em.offsets_of(lengths, 4).to(DEV)
+    g = seeded(t)
+    x, grad = em.small_integers((t, k), g, 1), em.small_integers((t, n), g, 1)
+    w = em.small_integers((len(lengths), n, k), g, 1)
+    x *= (torch.rand(x.shape, generator=g) < 0.2)
+    w *= (torch.rand(w.shape, generator=g) < 0.05)
+    grad[:, 100:] *= (torch.rand(grad[:, 100:].shape, generator=g) < 0.2)
+    dx, dw = grouped.gemm_grouped_bf16_backward(bf(grad), bf(x), bf(w), off)
+    used = slice(4, 4 + sum(lengths))
+    assert torch.equal(dx[used], grouped.gemm_grouped_bf16_grad_input(bf(grad), bf(w), off)[used])
+    assert torch.equal(dw, grouped.gemm_grouped_bf16_grad_weight(bf(grad), bf(x), off))
+    assert b.gemm_status() == 0
+    ends = off.tolist()
+    for e, (lo, hi) in enumerate(zip(ends[:-1], ends[1:])):
+        assert torch.equal(dx[lo:hi].float().cpu(), grad[lo:hi] @ w[e])
+        assert torch.equal(dw[e].float().cpu(), grad[lo:hi].t() @ x[lo:hi])
+
+
 def test_gradients_against_differences():
     """The forward product is linear in x and in W, so a difference of any size
     is the gradient's product with it; in small integers both are exact."""
