@@ -150,9 +150,9 @@ __device__ __forceinline__ bool elect_one() {
 // Bounded wait of a whole converged warp (mbar_wait is one thread's).  All
 // lanes poll with one instruction, read one flag and count alike, so that they
 // leave together; a count needs no registers for clocks, of which the e4m3
-// kernel's readers have none to spare.  2^20 polls are ~20 ms at the least,
+// kernel's readers have none to spare.  2^22 polls are ~80 ms at the least,
 // thousands of times what any of these waits takes.
-constexpr uint32_t kWarpWaitPolls = 1u << 20;
+constexpr uint32_t kWarpWaitPolls = 1u << 22;
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
