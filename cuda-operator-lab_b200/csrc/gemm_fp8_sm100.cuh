@@ -52,7 +52,7 @@ struct Fp8Cfg {
   static constexpr uint32_t kBBytes = BN / CG * kFp8BlockK;
   static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
   // k-blocks a stage
-  static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : (BN == 64 ? 4 : 2);
+  static constexpr int kKps = CG == 2 || kKBlockBytes > 40 * 1024 ? 1 : (BN == 64 ? 4 : 2);
   static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
   // one warp's sums of 32 rows, from each other CTA, for two warps
   static constexpr uint32_t kSumBytes = 32 * kCols * 4;

@@ -73,7 +73,9 @@ struct GroupedCfg {
   static constexpr uint32_t kABytes = ROWS * kBlockK * 2;
   static constexpr uint32_t kBBytes = BN / CG * kBlockK * 2;
   static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
-  static constexpr int kKps = kKBlockBytes > 40 * 1024 ? 1 : 2;  // k-blocks a stage
+  // k-blocks a stage: one for pairs (six stages; with three of two blocks 16384 rows
+  // over 8 experts, gate/up 4096 x 4096, took 758-766 us instead of 731-742)
+  static constexpr int kKps = CG == 2 || kKBlockBytes > 40 * 1024 ? 1 : 2;
   static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
   // 32 rows of 64 sums, from each other CTA, for two warps
   static constexpr uint32_t kSumBytes = 32 * 64 * 4;
