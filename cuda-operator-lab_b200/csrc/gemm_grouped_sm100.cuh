@@ -547,13 +547,18 @@ __device__ __forceinline__ void grouped_bf16_cta(const GroupedParams& p, int wor
         const int kb_begin = t.k_blocks * share / SPLIT;
         const int kb_end = t.k_blocks * (share + 1) / SPLIT;
         for (int kb = kb_begin; kb < kb_end; kb += kKps) {
-          if (!warp_wait(smem_u32(full_bar + stage), phase, abort_flag)) {
+          const int nk = min(kKps, kb_end - kb);
+          // The rows behind a ragged tail are zeroed by ordinary stores of both CTAs
+          // of a pair, so the wait that precedes their MMAs acquires at cluster scope.
+          const bool zeroed = CG == 2 && MODE == kGradW && kb + nk == t.k_blocks && ragged_rows(t) != 0;
+          const uint32_t full = smem_u32(full_bar + stage);
+          if (zeroed ? !warp_wait_cluster(full, phase, abort_flag)
+                     : !warp_wait(full, phase, abort_flag)) {
             if (lane == 0) fail(kStatusMma);
             ok = false;
             break;
           }
           tc_fence_after();
-          const int nk = min(kKps, kb_end - kb);
           if (elect_one()) {
 #pragma unroll
             for (int j = 0; j < kKps; ++j) {
