@@ -149,29 +149,63 @@ __device__ __forceinline__ bool elect_one() {
   return yes != 0;
 }
 
-// Bounded wait of a whole converged warp (mbar_wait is one thread's).  All
-// lanes poll with one instruction, read one flag and count alike, so that they
-// leave together; a count needs no registers for clocks, of which the e4m3
-// kernel's readers have none to spare.  2^22 polls are ~80 ms at the least,
-// thousands of times what any of these waits takes.
-constexpr uint32_t kWarpWaitPolls = 1u << 22;
+// Bounded waits of a whole converged warp (mbar_wait is one thread's).  All
+// lanes poll with one instruction and leave on one flag, so that they leave
+// together; the time limit sets that flag.  A wait that does not pass at once
+// keeps one 32-bit clock reading: the e4m3 kernel's readers have no registers
+// to spare.
+//
+// warp_wait is for what ends within one k-block or the storing of tiles: at most
+// the time of writing the whole output (~30 ms for all of the card's memory).
+// 2^31 cycles are 1.1 s at the highest clock.
+constexpr uint32_t kWarpWaitCycles = 1u << 31;
+
+__device__ __forceinline__ uint32_t clock32() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%clock;" : "=r"(t));
+  return t;
+}
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 63u) == 0u && *abort_flag) break;
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint32_t start = clock32();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock32() - start > kWarpWaitCycles) *abort_flag = 1;
   }
-  return false;
+  return true;
 }
 
 // warp_wait on data that other CTAs of the cluster wrote.
 __device__ __forceinline__ bool warp_wait_cluster(uint32_t bar, uint32_t parity,
                                                   volatile int* abort_flag) {
-  for (uint32_t i = 1; i < kWarpWaitPolls; ++i) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if ((i & 63u) == 0u && *abort_flag) break;
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const uint32_t start = clock32();
+  while (!mbar_try_wait_cluster(bar, parity)) {
+    if (*abort_flag) return false;
+    if (clock32() - start > kWarpWaitCycles) *abort_flag = 1;
   }
-  return false;
+  return true;
+}
+
+// Limit of a wait that spans the sums of whole tiles: a gradient by W sums over an
+// expert's rows, of which there may be 2^31 (2^25 k-blocks, several seconds).  A
+// k-block takes 0.3 to 0.8 us.
+__host__ __device__ constexpr unsigned long long blocks_limit_ns(unsigned long long k_blocks) {
+  return kWaitLimitNs + k_blocks * 20000ull;
+}
+
+// warp_wait over `k_blocks` k-blocks.
+__device__ __forceinline__ bool warp_wait_blocks(uint32_t bar, uint32_t parity,
+                                                 volatile int* abort_flag,
+                                                 unsigned long long k_blocks) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (*abort_flag) return false;
+    if (globaltimer_ns() - start > blocks_limit_ns(k_blocks)) *abort_flag = 1;
+  }
+  return true;
 }
 
 // Arrival on a barrier of the cluster that publishes no memory.
@@ -609,14 +643,17 @@ __device__ __forceinline__ void grouped_bf16_cta(const GroupedParams& p, int wor
       // ---------------- zeroes the rows behind a group's last one
       int stage = 0;  // slot of this tile's first stage
       uint32_t tail_phase = 0;  // bit s: parity of tail_bar[s]'s next completion
+      unsigned long long ahead = 0;  // k-blocks since the last tail: tiles without one are passed over
       for (int tile = worker; tile < num_tiles; tile += workers) {
         const GroupedTile t = grouped_tile<MODE, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
         const int stages = (t.k_blocks + kKps - 1) / kKps;
         const int first = ragged_rows(t);
+        ahead += t.k_blocks + 1;  // one for storing the tile
         if (first != 0) {
           const int slot = (stage + stages - 1) % kStages;
-          const bool got =
-              warp_wait(smem_u32(tail_bar + slot), (tail_phase >> slot) & 1u, abort_flag);
+          const bool got = warp_wait_blocks(smem_u32(tail_bar + slot), (tail_phase >> slot) & 1u,
+                                            abort_flag, ahead);
+          ahead = 0;
           tail_phase ^= 1u << slot;
           if (!got) {
             if (lane == 0) fail(kStatusProducer);
@@ -676,7 +713,8 @@ __device__ __forceinline__ void grouped_bf16_cta(const GroupedParams& p, int wor
         continue;
       }
       const int acc = local & 1;
-      if (!epi_wait(smem_u32(tfull_bar + acc), (local >> 1) & 1, abort_flag, lane)) {
+      if (!epi_wait(smem_u32(tfull_bar + acc), (local >> 1) & 1, abort_flag, lane,
+                    blocks_limit_ns(t.k_blocks))) {
         if (lane == 0) fail(kStatusEpilogue);
         break;
       }

@@ -252,11 +252,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // waits on whole tiles, so waking ~0.1 us late costs nothing, while 256
 // threads polling would take shared-memory and issue slots from the TMA and
 // MMA threads that share their SM sub-partitions.  __syncwarp orders the
-// other lanes after lane 0's acquire.  Same time limit as mbar_wait.
+// other lanes after lane 0's acquire.  Same time limit as mbar_wait, unless the
+// caller's tile may take longer.
 constexpr unsigned kEpiPollSleepNs = 64;
 
 __device__ __forceinline__ bool epi_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                         int lane) {
+                                         int lane, unsigned long long limit_ns = kWaitLimitNs) {
   int got = 0;
   if (lane == 0) {
     uint64_t t0 = 0;
@@ -271,7 +272,7 @@ __device__ __forceinline__ bool epi_wait(uint32_t bar, uint32_t parity, volatile
         const uint64_t now = globaltimer_ns();
         if (t0 == 0) {
           t0 = now;
-        } else if (now - t0 > kWaitLimitNs) {
+        } else if (now - t0 > limit_ns) {
           break;
         }
       }

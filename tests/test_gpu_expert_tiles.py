@@ -48,3 +48,29 @@ def test_weight_gradient_of_cta_pairs(lengths):
     for _ in range(5):
         assert torch.equal(grouped.gemm_grouped_bf16_grad_weight(grad, x, off), dw)
     assert b.gemm_status() == 0
+
+
+def test_sums_of_seconds_end_by_themselves():
+    """An expert of 3/4 of 2**30 rows: one CTA sums its only tile for seconds, its
+    warps that store it and that zero the next ragged tail wait all that time.  The
+    CTA's next tile is that of expert 148, whose 17 rows end inside a step of 16."""
+    many, n, k = 3 << 28, 8, 8
+    lengths = [many] + [0] * 147 + [17, 5]
+    t, off = sum(lengths), em.offsets_of(lengths).to(DEV)
+    g = seeded(90)
+    x = torch.zeros(t, k, device=DEV, dtype=torch.bfloat16)
+    grad = torch.zeros(t, n, device=DEV, dtype=torch.bfloat16)
+    some = torch.randint(0, many, (200,), generator=g).unique()
+    some = torch.cat([some, torch.tensor([many - 1]), torch.arange(many, t)]).unique()
+    xs = em.small_integers((len(some), k), g, 1)
+    gs = em.small_integers((len(some), n), g, 1)
+    x[some.to(DEV)] = xs.bfloat16().to(DEV)
+    grad[some.to(DEV)] = gs.bfloat16().to(DEV)
+    dw = grouped.gemm_grouped_bf16_grad_weight(grad, x, off)
+    assert b.gemm_status() == 0
+    del x, grad
+    dw = dw.float().cpu()
+    for e, lo, hi in ((0, 0, many), (148, many, many + 17), (149, many + 17, t)):
+        mine = (some >= lo) & (some < hi)
+        assert torch.equal(dw[e], gs[mine].t() @ xs[mine])
+    assert not dw[1:148].any()
