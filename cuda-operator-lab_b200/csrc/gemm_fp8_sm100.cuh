@@ -10,12 +10,14 @@
 // sums rotate through 512 / BN accumulators, so the MMAs of the next blocks run
 // while eight warps read one: a thread owns one row, whose activation scale is
 // a scalar, and BN / 2 columns inside one 128-row block of w, whose weight
-// scale is a scalar too, so a block costs one multiply-add an element.
+// scale is a scalar too, so a block costs one multiply-add an element (where the
+// scales' product is no normal number, two multiplications: block_scale.cuh).
 //
 // Roles, tiles, ragged edges and bounded waits are those of the bf16 kernel
 // (gemm_grouped_sm100.cuh); a dense product is one group of all rows.
 #pragma once
 
+#include "block_scale.cuh"
 #include "gemm_grouped_sm100.cuh"
 
 namespace col {
@@ -126,6 +128,19 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
                  "+r"(r[30]), "+r"(r[31])
                :
                : "memory");
+}
+
+// 16 columns back to TMEM; tmem_st_wait completes them.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
@@ -447,18 +462,16 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
         constexpr int kChunks = kCols / kChunk;
         static_assert(kChunks % 2 == 0, "the chunks' registers alternate");
         int in_group = 0;
-        auto chunk_addr = [&](int c) {
-          uint32_t col;
-          if constexpr (SWIGLU) {
-            // this thread's gate columns, then the up columns of the same outputs
-            constexpr int kGate = kCols / 2;
-            col = c * kChunk < kGate ? part_of * kGate + c * kChunk
-                                     : BN / 2 + part_of * kGate + c * kChunk - kGate;
-          } else {
-            col = part_of * kCols + c * kChunk;
-          }
+        // TMEM address of this thread's column `mine` of the sum: with SWIGLU its
+        // gate columns, then the up columns of the same outputs.
+        auto column = [&](int mine) {
+          constexpr int kGate = kCols / 2;
+          const uint32_t col = !SWIGLU          ? part_of * kCols + mine
+                               : mine < kGate   ? part_of * kGate + mine
+                                                : BN / 2 + part_of * kGate + mine - kGate;
           return t_lane + (acc * kGroup + in_group) * BN + col;
         };
+        auto chunk_addr = [&](int c) { return column(c * kChunk); };
         // Plain loads: the kernel that writes the scales may still have been running
         // when this one started, which non-coherent loads do not allow for.
         float next_x = fp.a_scale[xs];
@@ -469,8 +482,29 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
         if (ok) tmem_ld_start(chunk_addr(0), part[0]);
 #pragma unroll 1
         for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
-          const float sw = next_x * next_w;
-          const float su = next_x * next_u;
+          float sw = next_x * next_w;
+          float su = next_x * next_u;
+          // One branch for the warp; a row's own result does not depend on it.
+          // Rare: the sum is multiplied by the first scale where it lies.
+          if (__any_sync(0xffffffffu, !normal_f32(sw) || (SWIGLU && !normal_f32(su)))) {
+            const BlockScales two = block_scales(next_x, next_w);
+            const BlockScales two_up = block_scales(next_x, next_u);
+            tmem_ld_wait(part[0]);
+#pragma unroll 1
+            for (int c = 0; c < kCols; c += 16) {
+              const float first = SWIGLU && c >= kCols / 2 ? two_up.first : two.first;
+              uint32_t piece[16];
+              tmem_ld_start(column(c), piece);
+              tmem_ld_wait(piece);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) piece[i] = __float_as_uint(__uint_as_float(piece[i]) * first);
+              tmem_st16(column(c), piece);
+            }
+            tmem_st_wait();
+            sw = two.rest;
+            su = two_up.rest;
+            tmem_ld_start(chunk_addr(0), part[0]);
+          }
           if (kb + 1 < kb_end) {
             next_x = fp.a_scale[++xs];
             next_w = fp.b_scale[++ws];

@@ -5,7 +5,8 @@
 //   kForward  out[r, j]   = sum_c x[r, c] w[g, j, c]        (SwiGLU: silu(gate) * up)
 //   kGradX    dx[r, c]    = sum_j dy[r, j] w[g, j, c]
 //   kGradW    dw[g, j, c] = sum_r dy[r, j] x[r, c]
-// e4m3 operands are multiplied by their block scales as they are staged.
+// e4m3 operands: each block of 128 is summed by itself and added times its two
+// scales, as on the tensor cores.
 // 64 x 64 output tile per 256-thread CTA, 16-deep slices through shared
 // memory, 4 x 4 fp32 sums a thread: bound by the fp32 FMA rate.
 #pragma once
@@ -15,6 +16,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "block_scale.cuh"
 #include "grouped_schedule.cuh"
 
 namespace col {
@@ -79,11 +81,38 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(const GroupedSimtPara
       float acc[4][4] = {};
       float up[4][4] = {};
       const std::size_t wbase = static_cast<std::size_t>(g) * p.w_rows;
-      const std::size_t sbase = static_cast<std::size_t>(g) * ((p.w_rows + 127) / 128);
-      auto load_w = [&](int row, int c) {
-        float v = grouped_elem<T>(p.b, (wbase + row) * p.k + c);
-        if constexpr (kScaled) v *= p.b_scale[(sbase + row / 128) * kb_count + c / 128];
-        return v;
+      auto load_w = [&](int row, int c) { return grouped_elem<T>(p.b, (wbase + row) * p.k + c); };
+      // e4m3: the sums of finished blocks
+      float total[kScaled ? 4 : 1][kScaled ? 4 : 1] = {};
+      float total_up[kScaled && SWIGLU ? 4 : 1][kScaled && SWIGLU ? 4 : 1] = {};
+      // The block with column c is summed.  64 columns of the tile lie in one
+      // 128-row block of w.
+      auto end_block = [&](int c) {
+        if constexpr (kScaled) {
+          const std::size_t sbase = static_cast<std::size_t>(g) * ((p.w_rows + 127) / 128);
+          const float w_scale = p.b_scale[(sbase + j0 / 128) * kb_count + c / 128];
+          float up_scale = 0.0f;
+          if constexpr (SWIGLU) up_scale = p.b_scale[(sbase + (p.n + j0) / 128) * kb_count + c / 128];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const std::size_t row = range.begin + min(i0 + ty * 4 + i, out_rows - 1);
+            const float x_scale = p.a_scale[row * kb_count + c / 128];
+            const BlockScales two = block_scales(x_scale, w_scale);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              total[i][j] = fmaf(acc[i][j] * two.first, two.rest, total[i][j]);
+              acc[i][j] = 0.0f;
+            }
+            if constexpr (SWIGLU) {
+              const BlockScales up_two = block_scales(x_scale, up_scale);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                total_up[i][j] = fmaf(up[i][j] * up_two.first, up_two.rest, total_up[i][j]);
+                up[i][j] = 0.0f;
+              }
+            }
+          }
+        }
       };
       for (int s0 = 0; s0 < depth; s0 += kSlice) {
         for (int e = threadIdx.x; e < kTile * kSlice; e += 256) {
@@ -95,7 +124,6 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(const GroupedSimtPara
               if constexpr (MODE == kForward) {
                 const std::size_t row = static_cast<std::size_t>(range.begin + i0 + r);
                 a = grouped_elem<T>(p.a, row * p.k + d);
-                if constexpr (kScaled) a *= p.a_scale[row * kb_count + d / 128];
               } else if constexpr (MODE == kGradX) {
                 a = grouped_elem<T>(p.a, static_cast<std::size_t>(range.begin + i0 + r) * p.n + d);
               } else {
@@ -130,6 +158,7 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(const GroupedSimtPara
           }
         }
         __syncthreads();
+        if (kScaled && ((s0 + kSlice) % 128 == 0 || s0 + kSlice >= depth)) end_block(s0);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -140,7 +169,11 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(const GroupedSimtPara
           if (r < out_rows && c < cols) {
             const std::size_t row = MODE == kGradW ? static_cast<std::size_t>(g) * p.n + r
                                                    : static_cast<std::size_t>(range.begin + r);
-            const float v = SWIGLU ? silu_f(acc[i][j]) * up[i][j] : acc[i][j];
+            float v = acc[i][j];
+            float u = up[i][j];
+            if constexpr (kScaled) v = total[i][j];
+            if constexpr (kScaled && SWIGLU) u = total_up[i][j];
+            if constexpr (SWIGLU) v = silu_f(v) * u;
             p.out[row * cols + c] = __float2bfloat16_rn(v);
           }
         }
