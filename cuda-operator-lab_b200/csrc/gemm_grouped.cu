@@ -247,24 +247,79 @@ int launch_grouped_bf16(GroupedParams& p, std::uint64_t most_tiles, int dev, int
                                 dim3(col::sm100::kCtaThreads), Cfg::kSmemBytes, s, p);
 }
 
-// The variant of a bf16 product with `columns` accumulator columns, and its time.
-template <int MODE>
-Variant choose_bf16(std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
-                    std::uint64_t columns, int sm_count, double* us_out = nullptr) {
+// The variant of a bf16 product by waves of tiles, and its time.
+Variant waves_bf16(int mode, std::uint64_t t, std::uint64_t k, std::uint64_t n,
+                   std::uint64_t experts, std::uint64_t columns, int sm_count,
+                   double* us_out = nullptr) {
   // Rows a group: of the operand that a tile's rows come from (kGradW: of w, the
   // same for every group, and the sums have T rows over the groups).
   const double group_rows = static_cast<double>(t) / static_cast<double>(t < experts ? t : experts);
-  const double k_blocks = MODE == kGradW   ? std::ceil(group_rows / 64.0)
-                          : MODE == kGradX ? std::ceil(static_cast<double>(n) / 64.0)
+  const double k_blocks = mode == kGradW   ? std::ceil(group_rows / 64.0)
+                          : mode == kGradX ? std::ceil(static_cast<double>(n) / 64.0)
                                            : std::ceil(static_cast<double>(k) / 64.0);
   return choose_variant(
       kBf16Costs,
       [&](int tile_rows) {
-        if (MODE == kGradW) return static_cast<double>(experts * ((n + tile_rows - 1) / tile_rows));
+        if (mode == kGradW) return static_cast<double>(experts * ((n + tile_rows - 1) / tile_rows));
         return expected_row_tiles(t, experts, false, tile_rows);
       },
-      static_cast<double>(columns), k_blocks, MODE == kGradW ? 1e9 : group_rows, sm_count,
-      MODE != kGradW, us_out);
+      static_cast<double>(columns), k_blocks, mode == kGradW ? 1e9 : group_rows, sm_count,
+      mode != kGradW, us_out);
+}
+
+// The variant that a bf16 product runs.
+Variant choose_bf16(int mode, bool swiglu, std::uint64_t t, std::uint64_t k, std::uint64_t n,
+                    std::uint64_t experts, int sm_count) {
+  const std::uint64_t columns = mode != kForward ? k : swiglu ? 2 * n : n;
+  Variant v = waves_bf16(mode, t, k, n, experts, columns, sm_count);
+  if (mode == kGradW) return v;
+  // A few tiles of few rows: four or two CTAs share each sum while there are SMs
+  // for them, with at least four k-blocks apiece.
+  const std::uint64_t tiles = most_row_tiles(t, experts, false, 32) * ((columns + 127) / 128);
+  const std::uint64_t k_blocks = ((mode == kForward ? k : n) + 63) / 64;
+  for (const int split : {4, 2}) {
+    if (v.split == 1 && tiles * split <= static_cast<std::uint64_t>(sm_count) &&
+        k_blocks >= 4u * split) {
+      v = Variant{1, 128, 32, split};
+    }
+  }
+  return v;
+}
+
+// Whether 32 bits count the scales.
+inline bool scales_ok(std::uint64_t t, std::uint64_t k, std::uint64_t w_rows, std::uint64_t experts) {
+  const std::uint64_t k_blocks = (k + 127) / 128;
+  return t * k_blocks <= kIntMax && experts * ((w_rows + 127) / 128) * k_blocks <= kIntMax;
+}
+
+// The variant that an e4m3 product runs; `known`: all rows are one group's.
+Variant choose_fp8(std::uint64_t t, std::uint64_t k, std::uint64_t w_rows, std::uint64_t experts,
+                   bool known, int sm_count) {
+  const std::uint64_t k_blocks = (k + 127) / 128;
+  const double used = static_cast<double>(t < experts ? t : experts);
+  Variant v = choose_variant(
+      kFp8Costs, [&](int tile_rows) { return expected_row_tiles(t, experts, known, tile_rows); },
+      static_cast<double>(w_rows), static_cast<double>(k_blocks), static_cast<double>(t) / used,
+      sm_count, false);
+  // A few tiles of few rows: four or two CTAs share each sum while there are
+  // SMs for them, with at least two k-blocks apiece.  One row by 4096 x 4096:
+  // 12.5 us with one CTA a tile, 9.1 with two, 8.1 with four; one row by 1024 x
+  // 4096: 12.2, 8.2, 6.9, and 6.2 with four and 64 columns.
+  const std::uint64_t tiles32 = most_row_tiles(t, experts, known, 32);
+  double best_blocks = 0.0;
+  for (const int bn : {64, 128}) {
+    for (const int split : {2, 4}) {
+      const std::uint64_t ctas = tiles32 * ((w_rows + bn - 1) / bn) * split;
+      if (ctas > static_cast<std::uint64_t>(sm_count) || k_blocks < 2u * split) continue;
+      // k-blocks of a CTA, those of 64 columns at 0.7 of the others' time
+      const double blocks = std::ceil(static_cast<double>(k_blocks) / split) * (bn == 64 ? 0.7 : 1.0);
+      if (best_blocks == 0.0 || blocks < best_blocks) {
+        best_blocks = blocks;
+        v = Variant{1, bn, 32, split};
+      }
+    }
+  }
+  return v;
 }
 
 // What a product's kernel gets, but for its tiles; -1 where TMA cannot address the
@@ -317,20 +372,7 @@ int grouped_bf16_tc(const void* a, const void* b, const std::int32_t* offsets, v
   GroupedParams p;
   int rc = grouped_params<MODE, SWIGLU>(p, a, b, offsets, out, t, k, n, experts, dev, info);
   if (rc != 0) return rc;
-  const std::uint64_t out_cols = MODE == kForward ? n : k;
-  Variant v = choose_bf16<MODE>(t, k, n, experts, SWIGLU ? 2 * out_cols : out_cols, info.sm_count);
-  if constexpr (MODE != kGradW) {
-    // A few tiles of few rows: four or two CTAs share each sum while there are SMs
-    // for them, with at least four k-blocks apiece.
-    const std::uint64_t tiles = most_row_tiles(t, experts, false, 32) *
-                                ((out_cols * (SWIGLU ? 2 : 1) + 127) / 128);
-    for (const int split : {4, 2}) {
-      if (v.split == 1 && tiles * split <= static_cast<std::uint64_t>(info.sm_count) &&
-          p.num_k_blocks >= 4 * split) {
-        v = Variant{1, 128, 32, split};
-      }
-    }
-  }
+  const Variant v = choose_bf16(MODE, SWIGLU, t, k, n, experts, info.sm_count);
   rc = grouped_maps<MODE, SWIGLU>(p, v, a, b, t, k, n, experts);
   if (rc != 0) return rc;
   const int tile_rows = v.cg * v.rows;
@@ -372,11 +414,15 @@ int launch_backward(const GroupedParams& by_x, const GroupedParams& by_w, int in
 constexpr double kSecondLaunchUs = 4.0;
 constexpr double kBothMargin = 1.2;
 
-int backward_tc(const void* grad, const void* x, const void* w, const std::int32_t* offsets,
-                void* dx, void* dw, std::uint64_t t, std::uint64_t k, std::uint64_t n,
-                std::uint64_t experts, cudaStream_t s) {
-  int dev = 0;
-  const col::DeviceInfo& info = col::device_info(&dev);
+// The CTAs of either gradient in one launch; rows == 0: two launches take less.
+struct BothGradients {
+  int rows;  // of a tile of the gradient by x
+  int input_ctas;
+  int weight_ctas;
+};
+
+BothGradients plan_both(std::uint64_t t, std::uint64_t k, std::uint64_t n, std::uint64_t experts,
+                        int sm_count) {
   const std::uint64_t columns = (k + 127) / 128;
   const int rows = t <= 32 * experts ? 32 : 128;
   const double group_rows = static_cast<double>(t) / static_cast<double>(t < experts ? t : experts);
@@ -387,28 +433,37 @@ int backward_tc(const void* grad, const void* x, const void* w, const std::int32
   const double weight_us = std::ceil(group_rows / 64.0) * 0.285 + 0.8;
   double input_share = input_tiles;
   double weight_share = weight_tiles;
-  if (input_tiles + weight_tiles > info.sm_count) {
+  if (input_tiles + weight_tiles > sm_count) {
     const double part = input_tiles * input_us / (input_tiles * input_us + weight_tiles * weight_us);
-    input_share = std::fmin(std::fmax(std::round(part * info.sm_count), 1.0), info.sm_count - 1.0);
-    weight_share = info.sm_count - input_share;
+    input_share = std::fmin(std::fmax(std::round(part * sm_count), 1.0), sm_count - 1.0);
+    weight_share = sm_count - input_share;
   }
   const double both_us = std::fmax(std::ceil(input_tiles / input_share) * input_us,
                                    std::ceil(weight_tiles / weight_share) * weight_us);
   double first_us = 0.0;
   double second_us = 0.0;
-  choose_bf16<kGradX>(t, k, n, experts, k, info.sm_count, &first_us);
-  choose_bf16<kGradW>(t, k, n, experts, k, info.sm_count, &second_us);
-  if (both_us * kBothMargin >= first_us + second_us + kSecondLaunchUs) return -1;
+  waves_bf16(kGradX, t, k, n, experts, k, sm_count, &first_us);
+  waves_bf16(kGradW, t, k, n, experts, k, sm_count, &second_us);
+  if (both_us * kBothMargin >= first_us + second_us + kSecondLaunchUs) return {0, 0, 0};
+  return {rows, static_cast<int>(std::ceil(input_share)), static_cast<int>(weight_share)};
+}
+
+int backward_tc(const void* grad, const void* x, const void* w, const std::int32_t* offsets,
+                void* dx, void* dw, std::uint64_t t, std::uint64_t k, std::uint64_t n,
+                std::uint64_t experts, cudaStream_t s) {
+  int dev = 0;
+  const col::DeviceInfo& info = col::device_info(&dev);
+  const BothGradients plan = plan_both(t, k, n, experts, info.sm_count);
+  const int rows = plan.rows;
+  if (rows == 0) return -1;
   GroupedParams by_x, by_w;
   int rc = grouped_params<kGradX, false>(by_x, grad, w, offsets, dx, t, k, n, experts, dev, info);
   if (rc == 0) rc = grouped_params<kGradW, false>(by_w, grad, x, offsets, dw, t, k, n, experts, dev, info);
   if (rc == 0) rc = grouped_maps<kGradX, false>(by_x, {1, 128, rows, 1}, grad, w, t, k, n, experts);
   if (rc == 0) rc = grouped_maps<kGradW, false>(by_w, {1, 128, 128, 1}, grad, x, t, k, n, experts);
   if (rc != 0) return rc;
-  const int input_ctas = static_cast<int>(std::ceil(input_share));
-  const int weight_ctas = static_cast<int>(weight_share);
-  if (rows == 32) return launch_backward<32>(by_x, by_w, input_ctas, weight_ctas, dev, s);
-  return launch_backward<128>(by_x, by_w, input_ctas, weight_ctas, dev, s);
+  if (rows == 32) return launch_backward<32>(by_x, by_w, plan.input_ctas, plan.weight_ctas, dev, s);
+  return launch_backward<128>(by_x, by_w, plan.input_ctas, plan.weight_ctas, dev, s);
 }
 
 template <bool SWIGLU, int CG, int BN, int ROWS, int SPLIT>
@@ -451,7 +506,7 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
   const std::uint64_t k_blocks = (k + 127) / 128;
   const std::uint64_t scale_rows = (w_rows + 127) / 128;
   if (!tma_ok(x, k, 1) || !tma_ok(w, k, 1)) return -1;
-  if (t * k_blocks > kIntMax || experts * scale_rows * k_blocks > kIntMax) return -1;
+  if (!scales_ok(t, k, w_rows, experts)) return -1;
   int dev = 0;
   const col::DeviceInfo& info = col::device_info(&dev);
   if (info.cc_major != 10) return col::kErrDeviceNotSupported;
@@ -472,30 +527,7 @@ int fp8_tc(const void* x, const float* xs, const void* w, const float* ws,
   fp.b_scale = ws;
   fp.b_scale_rows = static_cast<int>(scale_rows);
 
-  const double used = static_cast<double>(t < experts ? t : experts);
-  Variant v = choose_variant(
-      kFp8Costs,
-      [&](int tile_rows) { return expected_row_tiles(t, experts, offsets == nullptr, tile_rows); },
-      static_cast<double>(w_rows), static_cast<double>(k_blocks), static_cast<double>(t) / used,
-      info.sm_count, false);
-  // A few tiles of few rows: four or two CTAs share each sum while there are
-  // SMs for them, with at least two k-blocks apiece.  One row by 4096 x 4096:
-  // 12.5 us with one CTA a tile, 9.1 with two, 8.1 with four; one row by 1024 x
-  // 4096: 12.2, 8.2, 6.9, and 6.2 with four and 64 columns.
-  const std::uint64_t tiles32 = most_row_tiles(t, experts, offsets == nullptr, 32);
-  double best_blocks = 0.0;
-  for (const int bn : {64, 128}) {
-    for (const int split : {2, 4}) {
-      const std::uint64_t ctas = tiles32 * ((w_rows + bn - 1) / bn) * split;
-      if (ctas > static_cast<std::uint64_t>(info.sm_count) || k_blocks < 2u * split) continue;
-      // k-blocks of a CTA, those of 64 columns at 0.7 of the others' time
-      const double blocks = std::ceil(static_cast<double>(k_blocks) / split) * (bn == 64 ? 0.7 : 1.0);
-      if (best_blocks == 0.0 || blocks < best_blocks) {
-        best_blocks = blocks;
-        v = Variant{1, bn, 32, split};
-      }
-    }
-  }
+  const Variant v = choose_fp8(t, k, w_rows, experts, offsets == nullptr, info.sm_count);
   p.num_n_blocks = static_cast<int>((w_rows + v.bn - 1) / v.bn);
   const std::uint64_t most_tiles =
       most_row_tiles(t, experts, offsets == nullptr, v.cg * v.rows) * p.num_n_blocks;
@@ -680,4 +712,51 @@ COL_API int cuda_operator_gemm_grouped_swiglu_fp8_block128(
   if (!offsets) return static_cast<int>(cudaErrorInvalidValue);
   return forward_fp8<true>(input_fp8, input_scale, packed_weight_fp8, weight_scale, offsets,
                            output_bf16, t, k, n, experts, stream);
+}
+
+COL_API int cuda_operator_lab_expert_tiles(int product, uint64_t t, uint64_t k, uint64_t n,
+                                           uint64_t experts, int sm_count, int* tiles) {
+  if (!tiles || sm_count < 2 || t == 0 || n == 0 || experts == 0 || !sizes_ok(t, k, n, experts)) {
+    return static_cast<int>(cudaErrorInvalidValue);
+  }
+  Variant v = {0, 0, 0, 0};
+  const bool k8 = k % 8 == 0;
+  const bool n8 = n % 8 == 0;
+  const std::uint64_t w_rows =
+      product == COL_EXPERT_SWIGLU_FP8 || product == COL_DENSE_SWIGLU_FP8 ? 2 * n : n;
+  const bool fp8 = k % 16 == 0 && scales_ok(t, k, w_rows, experts);
+  switch (product) {
+    case COL_EXPERT_BF16:
+    case COL_EXPERT_SWIGLU_BF16:
+      if (k8) v = choose_bf16(kForward, product == COL_EXPERT_SWIGLU_BF16, t, k, n, experts, sm_count);
+      break;
+    case COL_EXPERT_GRAD_INPUT:
+      if (k8 && n8) v = choose_bf16(kGradX, false, t, k, n, experts, sm_count);
+      break;
+    case COL_EXPERT_GRAD_WEIGHT:
+      if (k8 && n8) v = choose_bf16(kGradW, false, t, k, n, experts, sm_count);
+      break;
+    case COL_EXPERT_BOTH_GRADS:
+      if (k8 && n8) {
+        const int rows = plan_both(t, k, n, experts, sm_count).rows;
+        if (rows != 0) v = {1, 128, rows, 1};
+      }
+      break;
+    case COL_EXPERT_FP8:
+    case COL_EXPERT_SWIGLU_FP8:
+      if (fp8) v = choose_fp8(t, k, w_rows, experts, false, sm_count);
+      break;
+    case COL_DENSE_FP8:
+    case COL_DENSE_SWIGLU_FP8:
+      if (experts != 1) return static_cast<int>(cudaErrorInvalidValue);
+      if (fp8) v = choose_fp8(t, k, w_rows, 1, true, sm_count);
+      break;
+    default:
+      return static_cast<int>(cudaErrorInvalidValue);
+  }
+  tiles[0] = v.cg;
+  tiles[1] = v.bn;
+  tiles[2] = v.rows;
+  tiles[3] = v.split;
+  return 0;
 }

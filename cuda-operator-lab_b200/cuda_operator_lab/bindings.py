@@ -105,6 +105,7 @@ _SIGNATURES["cuda_operator_gemm_grouped_bf16_backward"] = [
 for _v in ("input", "weight"):
     _SIGNATURES[f"cuda_operator_gemm_grouped_bf16_grad_{_v}"] = [
         _P, _P, _P, _P, _U64, _U64, _U64, _U64, _P]
+_SIGNATURES["cuda_operator_lab_expert_tiles"] = [_I32, _U64, _U64, _U64, _U64, _I32, _P]
 _SIGNATURES["cuda_operator_lab_reduction_noalloc"] = [_P, _P, _U64, _P]
 
 _RESTYPES = {
@@ -1285,6 +1286,28 @@ def device_info() -> dict[str, int]:
     _call("cuda_operator_lab_device_info", ctypes.byref(sm), ctypes.byref(major),
           ctypes.byref(minor))
     return {"sm_count": sm.value, "cc_major": major.value, "cc_minor": minor.value}
+
+
+#: Products of :func:`expert_tiles`, in the order of the header's numbers.
+EXPERT_PRODUCTS = ("bf16", "swiglu_bf16", "grad_input", "grad_weight", "both_grads",
+                   "fp8", "swiglu_fp8", "dense_fp8", "dense_swiglu_fp8")
+
+
+def expert_tiles(product: str, t: int, k: int, n: int, experts: int = 1,
+                 sm_count: int | None = None) -> tuple[int, int, int, int] | None:
+    """Tiles that an expert-layer product of ``fp8`` or ``grouped`` is computed in.
+
+    ``(CTAs of a tile, columns, rows of a CTA, CTAs that share a sum)`` on a device
+    of ``sm_count`` SMs (the current one's if not given), for aligned operands;
+    ``None`` where the CUDA cores compute it, and for ``both_grads`` also where
+    they are two launches.
+    """
+    if sm_count is None:
+        sm_count = device_info()["sm_count"]
+    tiles = (ctypes.c_int * 4)()
+    _call("cuda_operator_lab_expert_tiles", EXPERT_PRODUCTS.index(product), t, k, n, experts,
+          sm_count, tiles)
+    return tuple(tiles) if tiles[0] else None
 
 
 def build_tag() -> str:

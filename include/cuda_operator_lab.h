@@ -332,6 +332,25 @@ int cuda_operator_gemm_grouped_bf16_grad_weight(const void* grad_bf16, const voi
 /* Both of them, in one launch where the product is small. */
 int cuda_operator_gemm_grouped_bf16_backward(const void* grad_bf16, const void* input_bf16, const void* weight_bf16, const int32_t* offsets, void* grad_input_bf16, void* grad_weight_bf16, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, void* stream);
 
+/* Which tiles the tensor cores compute a product of an expert layer in, on a
+ * device of sm_count SMs, for operands on 16-byte boundaries: tiles[0] CTAs of a
+ * tile, [1] its columns, [2] its rows in each CTA, [3] CTAs that share its sum.
+ * All zero: the CUDA cores compute it; for both gradients also: two launches
+ * after one another.  The sizes are those of the product's own call; 0 rows,
+ * columns or experts are invalid.  Host-only, enqueues nothing. */
+enum {
+  COL_EXPERT_BF16 = 0,
+  COL_EXPERT_SWIGLU_BF16 = 1,
+  COL_EXPERT_GRAD_INPUT = 2,
+  COL_EXPERT_GRAD_WEIGHT = 3,
+  COL_EXPERT_BOTH_GRADS = 4,
+  COL_EXPERT_FP8 = 5,
+  COL_EXPERT_SWIGLU_FP8 = 6,
+  COL_DENSE_FP8 = 7,
+  COL_DENSE_SWIGLU_FP8 = 8
+};
+int cuda_operator_lab_expert_tiles(int product, uint64_t t, uint64_t k, uint64_t n, uint64_t experts, int sm_count, int* tiles);
+
 /* Number of SMs of the current device and the library's build tag; lets a
  * caller check which library it loaded.  Host-only, enqueues nothing. */
 int cuda_operator_lab_device_info(int* sm_count, int* cc_major, int* cc_minor);

@@ -9,9 +9,10 @@ import pytest
 import torch
 
 import expert_math as em
+import expert_tiles as et
 from conftest import seeded
 from cuda_operator_lab import bindings as b
-from cuda_operator_lab import grouped
+from cuda_operator_lab import fp8, grouped
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -20,6 +21,54 @@ DEV = "cuda"
 def rows_of(lengths):
     ends = em.offsets_of(lengths).tolist()
     return [(e, slice(lo, hi)) for e, (lo, hi) in enumerate(zip(ends[:-1], ends[1:]))]
+
+
+def on_148_sms():
+    return b.device_info()["sm_count"] == et.SM_COUNT
+
+
+@pytest.mark.parametrize("product,tiles,t,experts,n,k", et.CASES)
+def test_each_tile_shape(product, tiles, t, experts, n, k):
+    if on_148_sms():
+        assert b.expert_tiles(product, t, k, n, experts) == tiles
+    g = seeded(t + n + k)
+    lengths = et.ragged(t, experts)
+    off = em.offsets_of(lengths).to(DEV)
+    swiglu = "swiglu" in product
+    x = (torch.randn(t, k, generator=g) * torch.exp(torch.randn(k, generator=g))).bfloat16().to(DEV)
+    grad = torch.randn(t, n, generator=g).bfloat16().to(DEV)
+    w = (torch.randn(experts, 2 * n if swiglu else n, k, generator=g) * k ** -0.5).bfloat16().to(DEV)
+    if "fp8" in product:
+        xq, xs = fp8.quantize_fp8_block128(x)
+        wq, ws = fp8.quantize_fp8_block128_weight(w)
+        if product.startswith("dense"):
+            gemm = fp8.gemm_swiglu_fp8_block128 if swiglu else fp8.gemm_fp8_block128
+            call = lambda: (gemm(xq, xs, wq[0], ws[0]),)  # noqa: E731
+        else:
+            gemm = grouped.gemm_grouped_swiglu_fp8_block128 if swiglu else grouped.gemm_grouped_fp8_block128
+            call = lambda: (gemm(xq, xs, wq, ws, off),)  # noqa: E731
+        xd, wd = xq.double() * em.spread(xs, 1, t, k), wq.double() * em.spread(ws, 128, *w.shape[1:])
+        wanted = [lambda e, r: em.product(xd[r], wd[e], swiglu)]
+    else:
+        by_x = lambda e, r: em.product(grad[r].double(), w[e].double().mT, False)  # noqa: E731
+        by_w = lambda e, r: em.product(grad[r].double().mT, x[r].double().mT, False)  # noqa: E731
+        call, wanted = {
+            "bf16": (lambda: (grouped.gemm_grouped_bf16(x, w, off),),
+                     [lambda e, r: em.product(x[r].double(), w[e].double(), False)]),
+            "swiglu_bf16": (lambda: (grouped.gemm_grouped_swiglu_bf16(x, w, off),),
+                            [lambda e, r: em.product(x[r].double(), w[e].double(), True)]),
+            "grad_input": (lambda: (grouped.gemm_grouped_bf16_grad_input(grad, w, off),), [by_x]),
+            "grad_weight": (lambda: (grouped.gemm_grouped_bf16_grad_weight(grad, x, off),), [by_w]),
+            "both_grads": (lambda: grouped.gemm_grouped_bf16_backward(grad, x, w, off), [by_x, by_w]),
+        }[product]
+    got = call()
+    assert b.gemm_status() == 0
+    for y, want in zip(got, wanted):
+        of_experts = y.ndim == 3
+        for e, r in rows_of(lengths):
+            em.assert_within(y[e] if of_experts else y[r], *want(e, r))
+    again = call()
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
 
 
 @pytest.mark.parametrize("lengths", [
