@@ -5,12 +5,16 @@ Tolerances are those of expert_math (derived there).
 
 from __future__ import annotations
 
+import json
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import expert_math as em
 import expert_tiles as et
-from conftest import seeded
+from conftest import PACKAGE_DIR, seeded
 from cuda_operator_lab import bindings as b
 from cuda_operator_lab import fp8, grouped
 
@@ -69,6 +73,64 @@ def test_each_tile_shape(product, tiles, t, experts, n, k):
             em.assert_within(y[e] if of_experts else y[r], *want(e, r))
     again = call()
     assert all(torch.equal(p, q) for p, q in zip(got, again))
+
+
+def test_first_calls_of_each_set_up_inside_a_capture():
+    """Pairs ask how many fit the device and the wide e4m3 tiles how many registers they
+    start with, on their first call: it may be one that is captured."""
+    cases = [c for c in et.CASES if c[1] in (et.PAIRS, et.WIDE) and c[0] in
+             ("bf16", "swiglu_bf16", "grad_input", "grad_weight", "fp8", "swiglu_fp8", "dense_fp8")]
+    code = """
+import json, sys, torch
+sys.path.insert(0, sys.argv[1])
+from cuda_operator_lab import bindings, fp8, grouped
+E4M3 = torch.float8_e4m3fn
+prepared = []
+for product, t, experts, n, k, lengths in json.loads(sys.argv[2]):
+    rows = 2 * n if "swiglu" in product else n
+    off = torch.tensor([0] + lengths, dtype=torch.int32).cumsum(0).int().cuda()
+    if "fp8" in product:
+        kb, nb = -(-k // 128), -(-rows // 128)
+        x, w = torch.ones(t, k, device="cuda").to(E4M3), torch.ones(experts, rows, k, device="cuda").to(E4M3)
+        xs, ws = torch.full((t, kb), 0.5, device="cuda"), torch.full((experts, nb, kb), 0.5, device="cuda")
+        if product == "dense_fp8":
+            call = lambda a=(x, xs, w[0], ws[0]): fp8.gemm_fp8_block128(*a)
+        else:
+            f = grouped.gemm_grouped_swiglu_fp8_block128 if rows != n else grouped.gemm_grouped_fp8_block128
+            call = lambda f=f, a=(x, xs, w, ws, off): f(*a)
+        total, want = k / 4, None
+    else:
+        x = torch.ones(t, k, device="cuda", dtype=torch.bfloat16)
+        g = torch.ones(t, n, device="cuda", dtype=torch.bfloat16)
+        w = torch.ones(experts, rows, k, device="cuda", dtype=torch.bfloat16)
+        total, want = float(k), None
+        if product == "grad_input":
+            total, call = float(n), lambda a=(g, w, off): grouped.gemm_grouped_bf16_grad_input(*a)
+        elif product == "grad_weight":
+            want = torch.tensor(lengths).bfloat16().view(-1, 1, 1)
+            call = lambda a=(g, x, off): grouped.gemm_grouped_bf16_grad_weight(*a)
+        elif rows != n:
+            call = lambda a=(x, w, off): grouped.gemm_grouped_swiglu_bf16(*a)
+        else:
+            call = lambda a=(x, w, off): grouped.gemm_grouped_bf16(*a)
+    if want is None:  # silu(s) is s in bf16 for sums this large
+        want = torch.tensor(total * total if rows != n else total).bfloat16()
+    prepared.append((product, call, want.cuda()))
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    outs = [call() for _, call, _ in prepared]
+graph.replay()
+torch.cuda.synchronize()
+for (product, _, want), y in zip(prepared, outs):
+    assert (y == want).all(), product
+assert bindings.gemm_status() == 0
+print("captured")
+"""
+    sizes = [(p, t, experts, n, k, et.ragged(t, experts)) for p, _, t, experts, n, k in cases]
+    done = subprocess.run([sys.executable, "-c", code, str(PACKAGE_DIR), json.dumps(sizes)],
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stdout + done.stderr
 
 
 @pytest.mark.parametrize("lengths", [
