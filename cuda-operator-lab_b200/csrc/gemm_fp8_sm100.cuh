@@ -62,15 +62,11 @@ struct Fp8Cfg {
   static constexpr int kStagesFit =
       static_cast<int>((kSmemLimit - 1024 - kExtraBytes) / kStageBytes);
   static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
-  // Partial sums are handed over in groups: a whole stage's where TMEM holds two
-  // such groups, else one by one.  A hand-over costs the issuing warp ~300
-  // cycles (two waits, a commit) beside ~35 for each MMA.
-  static constexpr int kGroup = 512 / BN / kKps >= 2 ? kKps : 1;
-  static constexpr int kAccs = 512 / BN / kGroup;  // groups in flight
+  // A stage's partial sums are handed over together: two waits and a commit.
+  static constexpr int kAccs = 512 / BN / kKps;  // stages whose sums TMEM holds
   static constexpr uint32_t kSmemBytes = kStages * kStageBytes + 1024 + kExtraBytes;
-  static constexpr int kSlots = kStages * kKps / kGroup;  // groups in the ring
-  static_assert(kSlots >= kAccs && kSlots <= 32, "a slot outlives its partial sum");
-  static_assert((kStages + kSlots + kAccs + 3) * 8 + 8 <= 512 && kKps / kGroup <= 2, "barrier space");
+  static_assert(kAccs >= 2 && kStages >= kAccs, "a stage outlives its partial sums");
+  static_assert((2 * kStages + kAccs + 3) * 8 + 8 <= 512, "barrier space");
 };
 
 // Instruction descriptor, kind::f8f6f4: D fp32, A and B e4m3, both K-major.
@@ -176,8 +172,6 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
   constexpr int kStages = Cfg::kStages;
   constexpr int kKps = Cfg::kKps;
   constexpr int kAccs = Cfg::kAccs;
-  constexpr int kGroup = Cfg::kGroup;
-  constexpr int kGroups = kKps / kGroup;  // a stage
   constexpr uint32_t kIdesc = idesc_e4m3_f32(kBlockM * CG, BN);
   constexpr bool kSplitRegs = fp8_split_regs(BN);
 
@@ -186,13 +180,13 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
       (reinterpret_cast<std::uintptr_t>(smem_raw) + 1023) & ~static_cast<std::uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kStages * Cfg::kStageBytes);
   uint64_t* full_bar = bars;
-  // One barrier a group in the ring says that its MMAs are done: the warps that
-  // read the partial sums wait for it, and the producer before it refills the
-  // stage.  (A second commit for the producer cost ~0.1 us a block.)  No waiter
-  // can miss a phase: a slot is used again only after its partial sums were
-  // read, as there are at least as many slots as groups of accumulators.
+  // One barrier a stage says that its MMAs are done: the warps that read the
+  // partial sums wait for it, and the producer before it refills the stage.  (A
+  // second commit for the producer cost ~0.1 us a block.)  No waiter can miss a
+  // phase: a stage's MMAs are issued again only after its partial sums were
+  // read, as there are at least as many stages as sets of accumulators.
   uint64_t* done_bar = bars + kStages;
-  uint64_t* tempty_bar = done_bar + Cfg::kSlots;
+  uint64_t* tempty_bar = done_bar + kStages;
   uint64_t* drain_bar = tempty_bar + kAccs;
   uint64_t* sums_bar = drain_bar + 1;  // the other CTAs' sums for each of two warps
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(sums_bar + 2);
@@ -212,8 +206,10 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
   const int kb_end = p.num_k_blocks * (share + 1) / SPLIT;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(smem_u32(full_bar + s), 1);
-    for (int s = 0; s < Cfg::kSlots; ++s) mbar_init(smem_u32(done_bar + s), 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(full_bar + s), 1);
+      mbar_init(smem_u32(done_bar + s), 1);
+    }
     for (int a = 0; a < kAccs; ++a) mbar_init(smem_u32(tempty_bar + a), CG * kEpiWarps);
     mbar_init(smem_u32(drain_bar), 1);
     mbar_init(smem_u32(sums_bar), 1);
@@ -262,8 +258,6 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
       uint32_t phase = 0;
       uint32_t issued_mask = 0;
       uint32_t issued_phase = 0;
-      uint32_t slot_phase = 0;  // bit s: parity of slot s's next use
-      uint32_t last_slots = 0;  // two bits a stage: its last group in use
       int filled = 0;
       bool ok = true;
       for (int tile = worker; ok && tile < num_tiles; tile += workers) {
@@ -273,15 +267,10 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
         const bool whole = CG == 2 || rows == kBlockM;
         for (int kb = kb_begin; kb < kb_end; kb += kKps) {
           const int nk = min(kKps, kb_end - kb);
-          if (filled >= kStages) {
-            const int slot = stage * kGroups + static_cast<int>(last_slots >> (2 * stage) & 3u);
-            if (!warp_wait(smem_u32(done_bar + slot), ((slot_phase >> slot) & 1u) ^ 1u, abort_flag)) {
-              if (lane == 0) fail(kStatusProducer);
-              ok = false;
-              break;
-            }
-          } else {
-            ++filled;
+          if (filled >= kStages && !warp_wait(smem_u32(done_bar + stage), phase ^ 1u, abort_flag)) {
+            if (lane == 0) fail(kStatusProducer);
+            ok = false;
+            break;
           }
           if (elect_one()) {
             const uint32_t bytes = nk * ((whole ? kBlockM : rows) * 128u + Cfg::kBBytes);
@@ -312,12 +301,7 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
             }
           }
           __syncwarp();
-          const int last = (nk - 1) / kGroup;
-#pragma unroll
-          for (int i = 0; i < kGroups; ++i) {
-            if (i <= last) slot_phase ^= 1u << (stage * kGroups + i);
-          }
-          last_slots = (last_slots & ~(3u << (2 * stage))) | (static_cast<uint32_t>(last) << (2 * stage));
+          if (filled < kStages) ++filled;
           issued_mask |= 1u << stage;
           issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
           if (++stage == kStages) {
@@ -350,43 +334,38 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
         bool ok = true;
         bool issued_any = false;
         for (int tile = worker; ok && tile < num_tiles; tile += workers) {
-          for (int kb = kb_begin; ok && kb < kb_end; kb += kKps) {
+          for (int kb = kb_begin; kb < kb_end; kb += kKps) {
             if (!warp_wait(smem_u32(full_bar + stage), phase, abort_flag)) {
               if (lane == 0) fail(kStatusMma);
               ok = false;
               break;
             }
+            if (!warp_wait(smem_u32(tempty_bar + acc), acc_phase ^ 1u, abort_flag)) {
+              if (lane == 0) fail(kStatusMma);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-              if (kb + g * kGroup >= kb_end) break;
-              if (!warp_wait(smem_u32(tempty_bar + acc), acc_phase ^ 1u, abort_flag)) {
-                if (lane == 0) fail(kStatusMma);
-                ok = false;
-                break;
-              }
-              tc_fence_after();
-              if (elect_one()) {
+              for (int j = 0; j < kKps; ++j) {
+                if (j > 0 && kb + j >= kb_end) break;
+                const uint32_t d_tmem = tmem_base + (acc * kKps + j) * BN;
+                const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
+                const uint32_t sb = sa + Cfg::kABytes;
 #pragma unroll
-                for (int i = 0; i < kGroup; ++i) {
-                  const int j = g * kGroup + i;
-                  if (i > 0 && kb + j >= kb_end) break;
-                  const uint32_t d_tmem = tmem_base + (acc * kGroup + i) * BN;
-                  const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
-                  const uint32_t sb = sa + Cfg::kABytes;
-#pragma unroll
-                  for (int k = 0; k < kFp8BlockK / 32; ++k) {
-                    umma_e4m3<CG>(d_tmem, sdesc_kmajor_sw128(sa + k * 32),
-                                  sdesc_kmajor_sw128(sb + k * 32), kIdesc, k != 0 ? 1u : 0u);
-                  }
+                for (int k = 0; k < kFp8BlockK / 32; ++k) {
+                  umma_e4m3<CG>(d_tmem, sdesc_kmajor_sw128(sa + k * 32),
+                                sdesc_kmajor_sw128(sb + k * 32), kIdesc, k != 0 ? 1u : 0u);
                 }
-                grouped_commit<CG>(smem_u32(done_bar + stage * kGroups + g));
               }
-              __syncwarp();
-              issued_any = true;
-              if (++acc == kAccs) {
-                acc = 0;
-                acc_phase ^= 1u;
-              }
+              grouped_commit<CG>(smem_u32(done_bar + stage));
+            }
+            __syncwarp();
+            issued_any = true;
+            if (++acc == kAccs) {
+              acc = 0;
+              acc_phase ^= 1u;
             }
             if (++stage == kStages) {
               stage = 0;
@@ -414,8 +393,8 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
     const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
     const int kb_count = p.num_k_blocks;
     int acc = 0;
-    int slot = 0;
-    uint32_t slot_phase = 0;  // bit s: parity of slot s's next completion
+    int stage = 0;
+    uint32_t phase = 0;
     bool ok = true;
     for (int tile = worker; ok && tile < num_tiles; tile += workers) {
       const GroupedTile t = grouped_tile<kForward, SWIGLU, CG, BN, ROWS>(p, tables, tile, rank);
@@ -433,16 +412,12 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
       uint64_t sums[kCols / 2];  // two fp32 each
 #pragma unroll
       for (int i = 0; i < kCols / 2; ++i) sums[i] = 0u;
-      // The next group of partial sums: waits until its MMAs are done.
-      auto next_group = [&](int kb) {
-        if (!warp_wait(smem_u32(done_bar + slot), (slot_phase >> slot) & 1u, abort_flag)) return false;
-        slot_phase ^= 1u << slot;
-        // the group after it: the stage's other one, or the next stage's first
-        if (kGroups == 1 || (slot & 1) == 1 || kb + 1 == kb_end) {
-          slot = slot / kGroups * kGroups + kGroups;
-          if (slot == Cfg::kSlots) slot = 0;
-        } else {
-          ++slot;
+      // The next stage's partial sums: waits until its MMAs are done.
+      auto next_stage = [&]() {
+        if (!warp_wait(smem_u32(done_bar + stage), phase, abort_flag)) return false;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
         }
         tc_fence_after();
         return true;
@@ -453,15 +428,15 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
         if (++acc == kAccs) acc = 0;
       };
       if (!warp_ok) {
-        for (int kb = kb_begin; kb < kb_end; kb += kGroup) {
-          ok = next_group(kb);
+        for (int kb = kb_begin; kb < kb_end; kb += kKps) {
+          ok = next_stage();
           if (!ok) break;
           release();
         }
       } else {
         constexpr int kChunks = kCols / kChunk;
         static_assert(kChunks % 2 == 0, "the chunks' registers alternate");
-        int in_group = 0;
+        int in_stage = 0;
         // TMEM address of this thread's column `mine` of the sum: with SWIGLU its
         // gate columns, then the up columns of the same outputs.
         auto column = [&](int mine) {
@@ -469,7 +444,7 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
           const uint32_t col = !SWIGLU          ? part_of * kCols + mine
                                : mine < kGate   ? part_of * kGate + mine
                                                 : BN / 2 + part_of * kGate + mine - kGate;
-          return t_lane + (acc * kGroup + in_group) * BN + col;
+          return t_lane + (acc * kKps + in_stage) * BN + col;
         };
         auto chunk_addr = [&](int c) { return column(c * kChunk); };
         // Plain loads: the kernel that writes the scales may still have been running
@@ -478,7 +453,7 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
         float next_w = fp.b_scale[ws];
         float next_u = SWIGLU ? fp.b_scale[ws + wu] : 0.0f;
         uint32_t part[2][kChunk];
-        ok = next_group(kb_begin);
+        ok = next_stage();
         if (ok) tmem_ld_start(chunk_addr(0), part[0]);
 #pragma unroll 1
         for (int kb = kb_begin; ok && kb < kb_end; ++kb) {
@@ -514,18 +489,18 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
           for (int c = 0; c < kChunks; ++c) {
             tmem_ld_wait(part[c & 1]);
             // the next load is under way while this chunk is added: the next
-            // chunk of this sum, or the next sum's first, once this group is
-            // released where it ends
+            // chunk of this sum, or the next sum's first, once this stage's are
+            // released where they end
             if (c + 1 < kChunks) {
               tmem_ld_start(chunk_addr(c + 1), part[(c + 1) & 1]);
-            } else if (kGroup > 1 && in_group + 1 < kGroup && kb + 1 < kb_end) {
-              ++in_group;
+            } else if (kKps > 1 && in_stage + 1 < kKps && kb + 1 < kb_end) {
+              ++in_stage;
               tmem_ld_start(chunk_addr(0), part[0]);
             } else {
               release();
-              in_group = 0;
+              in_stage = 0;
               if (kb + 1 < kb_end) {
-                ok = next_group(kb + 1);
+                ok = next_stage();
                 if (ok) tmem_ld_start(chunk_addr(0), part[0]);
               }
             }
