@@ -162,21 +162,26 @@ struct VariantCost {
   double tile;
 };
 
-// bf16 (k-blocks of 64).  16384 rows over 8 experts, 4096 x 4096: pairs 398-467
-// us, single CTAs with 256 columns 451-489, with 128 columns 525.  256 rows over
-// 64 experts, gate/up 2048 x 4096: 32-row tiles 144-155 us, 128 columns 154-168,
-// 256 columns 159-164, pairs 222.
+// bf16 (k-blocks of 64); fastest of 12 runs of ten launches back to back on the same
+// inputs: 16384 rows over 8 experts, 4096 x 4096: pairs 376 us, single CTAs with 256
+// columns 476, with 128 columns 561.  256 rows over 64 experts, gate/up 2048 x
+// 4096: 32-row tiles 156 us, 128 columns 172, 256 columns 170, pairs 195.  Over 27
+// drawn sizes (512-16384 rows, 1-32 experts, widths 512-8192) the choice takes
+// 1.06 (forward), 1.08 (by x) and 1.06 (by W) times the best variant in the
+// geometric mean, at worst 1.5; pairs alone 1.09, 1.08 and 1.05, single CTAs 1.15
+// and more.  Below 128 rows a group pairs are not considered.
 constexpr VariantCost kBf16Costs[] = {
     {{2, 256, 128, 1}, 0.44, 0.53, 1.8},
     {{1, 256, 128, 1}, 0.48, 0.72, 1.4},
     {{1, 128, 128, 1}, 0.285, 0.38, 0.8},
     {{1, 128, 32, 1}, 0.285, 0.34, 0.8},
 };
+constexpr int kSingle128 = 2;
 
-// e4m3 (k-blocks of 128).  8192 x 4096 x 4096: pairs 133-150 us, 256 columns
-// 177, 128 columns 195; the decode shape above: 128 columns 85-100 us, 256
-// columns 87-91, pairs 127, 32-row tiles 97 (which therefore serve only sums
-// that a cluster shares).
+// e4m3 (k-blocks of 128), measured the same way: 8192 x 4096 x 4096: pairs 156 us,
+// 256 columns 192, 128 columns 205; the decode shape above: 128 columns 103 us,
+// 256 columns 112, pairs 161.  Tiles of 32 rows took as long as those of 128 there,
+// so they serve only sums that a cluster shares.
 constexpr VariantCost kFp8Costs[] = {
     {{2, 256, 128, 1}, 0.60, 0.66, 1.5},
     {{1, 256, 128, 1}, 0.79, 0.80, 1.5},
@@ -205,7 +210,7 @@ std::uint64_t most_row_tiles(std::uint64_t rows, std::uint64_t groups, bool know
 // `columns` (accumulator columns) span the tiles, `k_blocks` the sum of one.
 template <int COUNT, typename RowTiles>
 Variant choose_variant(const VariantCost (&costs)[COUNT], RowTiles row_tiles, double columns,
-                       double k_blocks, double rows_per_group, int sm_count, bool rows32,
+                       double k_blocks, double rows_per_group, int sm_count, bool rows32 = true,
                        double* us_out = nullptr) {
   Variant best = costs[0].v;
   double best_us = -1.0;
@@ -300,7 +305,7 @@ Variant choose_fp8(std::uint64_t t, std::uint64_t k, std::uint64_t w_rows, std::
   Variant v = choose_variant(
       kFp8Costs, [&](int tile_rows) { return expected_row_tiles(t, experts, known, tile_rows); },
       static_cast<double>(w_rows), static_cast<double>(k_blocks), static_cast<double>(t) / used,
-      sm_count, false);
+      sm_count);
   // A few tiles of few rows: four or two CTAs share each sum while there are
   // SMs for them, with at least two k-blocks apiece.  One row by 4096 x 4096:
   // 12.5 us with one CTA a tile, 9.1 with two, 8.1 with four; one row by 1024 x
@@ -408,11 +413,14 @@ int launch_backward(const GroupedParams& by_x, const GroupedParams& by_w, int in
 // less than two launches after one another; -1 where it does not, or TMA cannot
 // address the operands.  A second launch costs kSecondLaunchUs on the GPU (its
 // start, and the first one's last wave), and ~6 us of the caller's time.
-// 1100 rows over 20 experts, 520 x 776: 21.6 -> 16.6 us; 14 over 28, 216 x 184: 10.4
-// -> 5.5.  The margin is for shares that uneven groups unbalance: without it 3519
-// rows over 5, 2264 x 568, took 50.6 us instead of 39.6.
+// The margin is for shares that uneven groups unbalance: without it 3519 rows over
+// 5, 2264 x 568, took 50.6 us instead of 39.6.  Over 70 drawn sizes (8-6000 rows,
+// 1-64 experts, widths 64-3000, three spreads of the groups; back to back) the
+// choice takes 1.006 times the faster form in the geometric mean, at worst 1.20;
+// always two launches 1.43, at worst 2.04.
 constexpr double kSecondLaunchUs = 4.0;
 constexpr double kBothMargin = 1.2;
+constexpr double kInputBlockUs = 0.3;
 
 // The CTAs of either gradient in one launch; rows == 0: two launches take less.
 struct BothGradients {
@@ -428,9 +436,11 @@ BothGradients plan_both(std::uint64_t t, std::uint64_t k, std::uint64_t n, std::
   const double group_rows = static_cast<double>(t) / static_cast<double>(t < experts ? t : experts);
   const double input_tiles = expected_row_tiles(t, experts, false, rows) * static_cast<double>(columns);
   const double weight_tiles = static_cast<double>(experts * ((n + 127) / 128) * columns);
-  // a tile's time in either, as in kBf16Costs
-  const double input_us = std::ceil(static_cast<double>(n) / 64.0) * 0.3 + 0.8;
-  const double weight_us = std::ceil(group_rows / 64.0) * 0.285 + 0.8;
+  // a tile's time in either: of the single CTAs with 128 columns, whose blocks by x
+  // take between the two figures of the table, as part of the SMs read w
+  const VariantCost& cost = kBf16Costs[kSingle128];
+  const double input_us = std::ceil(static_cast<double>(n) / 64.0) * kInputBlockUs + cost.tile;
+  const double weight_us = std::ceil(group_rows / 64.0) * cost.block + cost.tile;
   double input_share = input_tiles;
   double weight_share = weight_tiles;
   if (input_tiles + weight_tiles > sm_count) {

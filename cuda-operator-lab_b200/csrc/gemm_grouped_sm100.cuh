@@ -74,7 +74,8 @@ struct GroupedCfg {
   static constexpr uint32_t kBBytes = BN / CG * kBlockK * 2;
   static constexpr uint32_t kKBlockBytes = kABytes + kBBytes;
   // k-blocks a stage: one for pairs (six stages; with three of two blocks 16384 rows
-  // over 8 experts, gate/up 4096 x 4096, took 758-766 us instead of 731-742)
+  // over 8 experts, gate/up 4096 x 4096, took 747-750 us instead of 738-745: fastest
+  // of 12 runs of ten launches back to back on the same inputs, measured twice)
   static constexpr int kKps = CG == 2 || kKBlockBytes > 40 * 1024 ? 1 : 2;
   static constexpr uint32_t kStageBytes = kKps * kKBlockBytes;
   // 32 rows of 64 sums, from each other CTA, for two warps
@@ -238,15 +239,15 @@ struct GroupedTile {
   int begin;    // the group's rows
   int end;
   int k_blocks;
-  int first_k;  // k-block that the sum starts with (few_rows_first_k)
 };
 
 // Tiles of few rows stream w from DRAM.  Started together, they would read the
 // same columns of all their rows, addresses that agree in their low bits, and
 // crowd on few channels; so each tile's sum starts at another (even, its stages
 // read pairs) k-block and wraps around.  256 rows over 64 experts, gate/up 2048
-// x 4096 in bf16: 157 -> 136 us.  It depends on the expert and the columns
-// alone, so a row's result does not depend on the other rows.
+// x 4096 in bf16, back to back on the same inputs: 161 -> 156 us.  It depends on
+// the expert, the columns and the tile's width, not on a tile's other rows (the
+// width is chosen from the sizes alone).
 __device__ __forceinline__ int few_rows_first_k(int group, int n_block, int num_n, int k_blocks) {
   const unsigned tile = static_cast<unsigned>(group) * num_n + n_block;
   return static_cast<int>(2u * (tile * 5u % ((k_blocks + 1u) / 2u)));
@@ -275,7 +276,6 @@ __device__ __forceinline__ GroupedTile grouped_tile(const GroupedParams& p, cons
   t.a_row = (MODE == kGradW ? 0 : t.begin) + c.m * kTileRows + rank * ROWS;
   t.col = c.n * (SWIGLU ? BN / 2 : BN);
   t.k_blocks = MODE == kGradW ? (t.end - t.begin + kBlockK - 1) / kBlockK : p.num_k_blocks;
-  t.first_k = ROWS == 32 ? few_rows_first_k(c.group, c.n, p.num_n_blocks, p.num_k_blocks) : 0;
   return t;
 }
 
@@ -468,6 +468,9 @@ __device__ __forceinline__ void grouped_bf16_cta(const GroupedParams& p, int wor
       const bool ragged = MODE == kGradW && ragged_rows(t) != 0;
       const int kb_begin = t.k_blocks * share / SPLIT;
       const int kb_end = t.k_blocks * (share + 1) / SPLIT;
+      const int first_k =
+          ROWS == 32 ? few_rows_first_k(t.group, t.col / (SWIGLU ? BN / 2 : BN), p.num_n_blocks, t.k_blocks)
+                     : 0;
       for (int kb = kb_begin; kb < kb_end; kb += kKps) {
         if (filled >= kStages && !warp_wait(smem_u32(empty_bar + stage), phase ^ 1u, abort_flag)) {
           if (lane == 0) fail(kStatusProducer);
@@ -496,7 +499,7 @@ __device__ __forceinline__ void grouped_bf16_cta(const GroupedParams& p, int wor
             if (j >= nk) break;
             const uint32_t sa = smem_u32(smem + stage * Cfg::kStageBytes + j * Cfg::kKBlockBytes);
             const uint32_t sb = sa + Cfg::kABytes;
-            int kc = kb + j + t.first_k;
+            int kc = kb + j + first_k;
             if (ROWS == 32 && kc >= t.k_blocks) kc -= t.k_blocks;
             kc *= kBlockK;
             if constexpr (MODE == kGradW) {

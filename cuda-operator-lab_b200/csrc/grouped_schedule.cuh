@@ -78,9 +78,11 @@ struct TileCoords {
 
 // Tile number to (group, row tile, column tile).  Within a group, kGroupRows
 // row tiles at a time walk the columns together, so that the tiles in flight
-// share operand rows and columns in L2.  32 against 16, 8 and 4: 8192 x 4096 x
-// 14336 SwiGLU in e4m3 896-935 us (931-937, 948-954, 943-970), 16384 rows over 8
-// experts, gate/up 4096 x 4096 in bf16, 742-750 us (767-770, 776, 768-790).
+// share operand rows and columns in L2.  With 32, 16, 8 and 4, fastest of 12
+// runs of ten launches back to back on the same inputs, measured twice: 16384 rows over 8 experts,
+// gate/up 4096 x 4096 in bf16, 738-745, 735-744, 744 and 748-753 us; 8192 x 4096 x
+// 14336 SwiGLU in e4m3 972-994, 925-985, 1028-1039 and 955-957 (single launches
+// up to 1400, as the clock falls): no difference between 16 and 32 shows.
 constexpr int kGroupRows = 32;
 
 __device__ __forceinline__ TileCoords tile_of(int tile, const int* prefix, int groups,

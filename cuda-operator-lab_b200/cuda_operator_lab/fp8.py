@@ -7,7 +7,9 @@ front where there are several).  For a block with largest magnitude ``a`` (at
 least 2**-100) the scale is ``a / 448`` and the values are ``x * 448 / a`` rounded
 to nearest even (of the exact quotient), so ``q.float() * scale`` stands for
 ``x``.  A NaN or
-an infinity in a block makes every product over that block NaN.
+an infinity in a block makes every product over that block NaN.  The products
+take any finite fp32 scales, also ones whose product overflows or underflows
+where the scaled sum does not.
 
 As in ``bindings``: contiguous CUDA tensors, the current stream of the
 operands' device, ``_into`` forms that return the caller's storage, no
