@@ -18,6 +18,10 @@ __device__ __forceinline__ bool normal_f32(float v) {
   return (__float_as_uint(v) << 1) - (0x00800000u << 1) < ((0x7f800000u - 0x00800000u) << 1);
 }
 
+__device__ __forceinline__ bool finite_nonzero(float v) {
+  return (__float_as_uint(v) << 1) - 1u < (0x7f800000u << 1) - 1u;
+}
+
 // p a b = (p first) rest
 struct BlockScales {
   float first;
@@ -26,8 +30,8 @@ struct BlockScales {
 
 __device__ __forceinline__ BlockScales block_scales(float a, float b) {
   const float product = a * b;
-  // a zero scale makes the product an exact zero (or NaN, beside an infinity)
-  if (normal_f32(product) || a == 0.0f || b == 0.0f) return {1.0f, product};
+  // a zero, an infinity or a NaN among the scales is in the product too
+  if (normal_f32(product) || !finite_nonzero(a) || !finite_nonzero(b)) return {1.0f, product};
   return fabsf(a) > fabsf(b) ? BlockScales{a, b} : BlockScales{b, a};
 }
 

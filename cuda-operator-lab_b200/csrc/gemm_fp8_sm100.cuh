@@ -465,8 +465,10 @@ __global__ void __cluster_dims__(CG * SPLIT, 1, 1) __launch_bounds__(kCtaThreads
             const BlockScales two = block_scales(next_x, next_w);
             const BlockScales two_up = block_scales(next_x, next_u);
             tmem_ld_wait(part[0]);
+            // (nothing to multiply where no scale but zeros, infinities and NaN is met)
+            const bool some = __any_sync(0xffffffffu, two.first != 1.0f || (SWIGLU && two_up.first != 1.0f));
 #pragma unroll 1
-            for (int c = 0; c < kCols; c += 16) {
+            for (int c = some ? 0 : kCols; c < kCols; c += 16) {
               const float first = SWIGLU && c >= kCols / 2 ? two_up.first : two.first;
               uint32_t piece[16];
               tmem_ld_start(column(c), piece);
