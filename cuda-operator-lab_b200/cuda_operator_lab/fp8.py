@@ -21,10 +21,14 @@ boundaries, elsewhere on a much slower CUDA-core kernel.
 from __future__ import annotations
 
 import torch
-from torch._C import _cuda_getDevice as _current_device
 
 from . import bindings
 from .bindings import _ptr, _stream
+
+try:
+    from torch._C import _cuda_getDevice as _current_device
+except ImportError:  # a torch without CUDA: every call is refused for its tensors
+    from torch.cuda import current_device as _current_device
 
 __all__ = [
     "quantize_fp8_block128", "quantize_fp8_block128_into",

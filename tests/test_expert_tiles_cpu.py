@@ -3,10 +3,13 @@
 from __future__ import annotations
 
 import ctypes
+import subprocess
+import sys
 
 import pytest
 
 import expert_tiles as et
+from conftest import PACKAGE_DIR
 from cuda_operator_lab import bindings as b
 from test_abi import library
 
@@ -65,3 +68,20 @@ def test_refusals():
     assert call(0, 1, 8, 8, 1, 1, tiles) == 1
     with pytest.raises(ValueError):
         b.expert_tiles("no such product", 1, 8, 8, 1, 148)
+
+
+def test_the_modules_import_under_a_torch_without_cuda():
+    """Such a torch has no device query in its C module; calls are refused, not the import."""
+    code = """
+import sys, torch
+del torch._C._cuda_getDevice
+sys.path.insert(0, sys.argv[1])
+from cuda_operator_lab import fp8, grouped
+try:
+    fp8.quantize_fp8_block128(torch.zeros(2, 128))
+except ValueError as exc:
+    assert "CUDA" in str(exc)
+    print("refused")
+"""
+    done = subprocess.run([sys.executable, "-c", code, str(PACKAGE_DIR)], capture_output=True, text=True)
+    assert done.returncode == 0 and "refused" in done.stdout, done.stderr
